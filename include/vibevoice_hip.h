@@ -642,6 +642,71 @@ vv_status_t vv_kv_unrotate_dev(void* x_fp16, int n_heads, int head_dim, int rows
 vv_status_t vv_kv_page_map_dev(int* page_table, int first, int n, const int* pages,
                                void* stream);
 
+/* ── Serving many sequences: one pool of pages, one launch a step (additions) ── */
+
+/* A pool is one layer's K and V stores [n_pages * 64][n_kv_heads][head_dim] as vv_kv_view_t describes them; page p
+ * holds rows 64 p .. 64 p + 63. Each of n_seqs sequences has a row of max_pages page ids (int32) in page_tables and
+ * its length in cache_lens: position t of sequence i lies in row ("slot")
+ * page_tables[i * max_pages + t / 64] * 64 + t % 64. Sequences may share pages that none of them writes. */
+
+/* addition: the pages and slots of a step's new positions, from the lengths, all on the device: sequence i holds
+ * cache_lens[i] positions and gets new_lens[i] more (<= 0: none), in ceil((len + new) / 64) - ceil(len / 64) new
+ * pages off the top of the stack free_pages[0 .. *n_free): page number j handed out, counting through the sequences in
+ * order and through each one's positions, is free_pages[*n_free - 1 - j]; its id goes into the sequence's table.
+ * A sequence is refused, gets nothing and keeps its length when its positions would not fit max_pages pages, when its
+ * rows would end past max_rows, when its length is negative, or when it needs pages and the running sum of needed
+ * pages (in order, those refused for want of pages counted: none overtakes) passes *n_free.
+ *   lens_out[n_seqs]       lengths after the step
+ *   row_starts[n_seqs + 1] first packed row of each sequence: the running sum of new_lens (refused ones included, so
+ *                          rows keep the places the caller packed them in), held at max_rows
+ *   positions, slots [max_rows]  of each packed row; 0 and -1 for rows of refused sequences and rows past the last
+ *   counts[3]              free pages left, rows in use (row_starts[n_seqs]), sequences refused
+ * free_pages is not written: the pages in use are its top counts-many, so the caller carries counts[0] as the next
+ * *n_free, and returns a finished sequence's pages by writing them back from free_pages[*n_free] on.
+ * lens_out may be cache_lens and counts may be n_free (a captured step that advances itself); one workgroup then fills
+ * all rows. lens_out == new_lens: VV_ERR_INVALID_ARG. Replaces vv_kv_page_map_dev and host-side slot arithmetic
+ * per sequence. */
+vv_status_t vv_kv_page_plan_dev(const int* new_lens, const int* cache_lens, int n_seqs, int* page_tables,
+                                int max_pages, const int* free_pages, const int* n_free, int* lens_out,
+                                int* row_starts, int* positions, int64_t* slots, int max_rows, int* counts,
+                                void* stream);
+
+/* addition: bias, rotary embedding and KV append of n_rows packed rows, each at its own position and slot (what
+ * vv_kv_page_plan_dev writes): q_out[r] = rope(q[r] + q_bias, positions[r]) (q_out may be q), and, into row slots[r] of
+ * the pool, rope(k[r] + k_bias, positions[r]) and v[r] + v_bias. q, q_out [n_rows][n_q_heads][head_dim], k, v
+ * [n_rows][n_kv_heads][head_dim] FP16; a bias may be NULL. Every step rounds to FP16 where the separate calls store:
+ * the bits are those of vv_bias_add_dev, vv_rope_qk_dev and vv_kv_store_dev (without a reference key) on each row.
+ * A row whose slot is negative or not below 64 * n_pages is skipped: nothing of it is read or written, q_out
+ * included. Slots must differ from one another; of two rows with one slot either may win, vector piece by piece.
+ * kv_format FP16: any even head_dim <= 256 and 2-byte alignment (head_dim 64 and 128 with everything 16-byte aligned
+ * take the vector kernel); FP8 E4M3 / E5M2: head_dim 128, 16-byte aligned tensors, 8-byte aligned stores. Other
+ * formats, shapes and alignments: VV_ERR_UNSUPPORTED. */
+vv_status_t vv_rope_kv_append_dev(const void* q, const void* k, const void* v, const void* q_bias,
+                                  const void* k_bias, const void* v_bias, const int* positions,
+                                  const int64_t* slots, void* q_out, void* k_store, void* v_store, int n_rows,
+                                  int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int kv_format,
+                                  float theta, void* stream);
+
+/* Scratch for vv_attn_decode_batch: grows by four bytes a sequence, not with the lengths. 0 for arguments that the
+ * call refuses. */
+size_t vv_attn_decode_batch_scratch_bytes(int n_seqs, int n_q_heads, int n_kv_heads, int head_dim);
+/* addition: vv_attn_decode for n_seqs sequences at once: out[i] = attention of the one query row q[i]
+ * [n_q_heads][head_dim] against the first cache_lens[i] positions behind row i of kv->page_table ([n_seqs][max_pages],
+ * required here). Lengths are read on the device, may differ as they like and size nothing on the host: a captured
+ * step replays at any lengths. The pages of all sequences and KV heads are dealt out evenly over the workgroups,
+ * whatever sequence they belong to; a row that several workgroups share is folded in page order, so a result
+ * does not depend on timing (its last bits depend on where the batch's pages were cut).
+ * cache_lens[i] <= 0: zeros. A length past 64 * max_pages is taken as that. Positions behind a page id outside
+ * [0, n_pages) count as masked; what the pool holds past a length or there is never used, NaN included.
+ * FP16 pools of head_dim 64 and 128 with q and the stores 16-byte aligned run on the matrix cores, any other
+ * head_dim <= 256 or alignment on a slower kernel that needs no scratch; FP8 E4M3 / E5M2: head_dim 128, the same
+ * alignment. TurboQuant formats: VV_ERR_UNSUPPORTED. scratch: vv_attn_decode_batch_scratch_bytes() of device memory,
+ * 16-byte aligned (smaller or unaligned: VV_ERR_INVALID_ARG); it needs no clearing, holds nothing between calls, and
+ * calls that overlap need one each. */
+vv_status_t vv_attn_decode_batch(int backend, const void* q, const vv_kv_view_t* kv, void* out, int n_q_heads,
+                                 int n_seqs, const int* cache_lens, int max_pages, int n_pages, void* scratch,
+                                 size_t scratch_bytes, void* stream);
+
 /* ── LM head ───────────────────────────────────────────────────────────── */
 
 /* logits[V] = W[V,K] x[K]; x, W FP16, FP32 accumulation, FP32 logits. Bound by

@@ -28,55 +28,17 @@
 #include <algorithm>
 #include <atomic>
 
-#include "vv_common.hpp"
+#include "attn_common.hpp"
 
 namespace vv {
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef h16 h16x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kPage = 64;            // positions per page (include/vibevoice/kv_quant.h:52)
 constexpr int kFormatFp16 = 0;       // VV_KV_FP16
 constexpr int kMaxParts = 256;       // decode slices per KV head
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // The slack of a row's reference exponent below its running maximum, in base-2 exponents (RowState).
 constexpr float kMaxSlack = 8.0f;
-// A value and its partner's, 32 (or 16) lanes away, combined in the vector ALU: the gfx950 lane swaps exchange
-// the odd rows of one register with the even rows of another (rows of 32 or 16 lanes), so from two copies of v
-// one register ends up with the lower row's values in both rows of a pair and the other with the upper row's.
-// No trip through the LDS crossbar and no counter to wait for; max and + commute, so every lane gets the bits
-// that v (op) shuffle-xor(v) gave it. (As instructions: the compiler's builtin for them hands back the first
-// register twice. The two wait states are what it puts between a vector write and a swap that reads it.)
-__device__ __forceinline__ void swap_rows32(float& a, float& b) {
-    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-}
-__device__ __forceinline__ void swap_rows16(float& a, float& b) {
-    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-}
-__device__ __forceinline__ float max_xor32(float v) {
-    float a = v, b = v;
-    swap_rows32(a, b);
-    return fmaxf(a, b);
-}
-__device__ __forceinline__ float sum_xor32(float v) {
-    float a = v, b = v;
-    swap_rows32(a, b);
-    return a + b;
-}
-__device__ __forceinline__ float max_xor16(float v) {
-    float a = v, b = v;
-    swap_rows16(a, b);
-    return fmaxf(a, b);
-}
-__device__ __forceinline__ float sum_xor16(float v) {
-    float a = v, b = v;
-    swap_rows16(a, b);
-    return a + b;
-}
 
 __device__ __forceinline__ int cache_row(const int* page_table, int t) {
     return page_table ? page_table[t / kPage] * kPage + t % kPage : t;
@@ -179,11 +141,6 @@ struct TileRegs {
     Chunk k[kIter], v[kIter];
 };
 
-// Cache formats the matrix-core kernels read (include/vibevoice/kv_quant.h:34-36).
-// The FP8 ones are widened to FP16 on their way into the registers: every
-// E4M3 / E5M2 value is an FP16 value, so from there on the tile is the tile of
-// an FP16 cache that holds the decoded values.
-constexpr int kFmtFp16 = 0, kFmtE4M3 = 1, kFmtE5M2 = 2;
 // TurboQuant (kv_quant.h:37-40): 4, 3, 2 or 1.5 bits per value as one little-endian
 // bit stream per vector, value d at bit d * bits (pair P at bit 3 P for 1.5 bits),
 // each code an index into a table of Lloyd-Max levels of a unit Gaussian, times
@@ -209,24 +166,6 @@ template <int kFmt> struct KvFormat {
     static constexpr int kPerCode = kFmt == kFmtTq15 ? 2 : 1;
     static constexpr int kSlotBits = 8 / kPerCode * kCodeBits;
 };
-
-// Four FP8 codes (the bytes of `codes`) as two half2 words, lanes in byte order.
-template <int kFmt>
-__device__ __forceinline__ void widen4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
-    // byte b -> 16-bit lane b << 8: an E5M2 code IS the top byte of the FP16 value
-    lo = __builtin_amdgcn_perm(0u, codes, 0x010C000Cu);
-    hi = __builtin_amdgcn_perm(0u, codes, 0x030C020Cu);
-    if constexpr (kFmt == kFmtE4M3) {
-        // sign stays, exponent and mantissa move down one bit (FP16 has five exponent bits):
-        // that reads 2^-8 too small (bias 15 against 7), subnormals included, so scale by 256
-        typedef h16 h16x2v __attribute__((ext_vector_type(2)));
-        const h16x2v k256 = {(h16)256.0f, (h16)256.0f};
-        const uint32_t l = ((lo >> 1) & 0x3F803F80u) | (lo & 0x80008000u);
-        const uint32_t h = ((hi >> 1) & 0x3F803F80u) | (hi & 0x80008000u);
-        lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h16x2v, l) * k256);
-        hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h16x2v, h) * k256);
-    }
-}
 
 // `count` bits at bit `offset` of a vector of `nwords` 32-bit words.
 __device__ __forceinline__ uint32_t stream_bits(const uint32_t* __restrict__ words, int nwords, int offset,
@@ -1255,37 +1194,6 @@ __global__ __launch_bounds__(kBlock) void kv_store_fp16_chunks(
 }
 
 // ── FP8 cache store (src/cuda/kv_quant.cu:57-84, kv_codec.cuh:66-128) ──────
-// One value to E4M3 (bias 7, largest finite 448 = 0x7E) or E5M2 (bias 15,
-// largest finite 57344 = 0x7B) in integer arithmetic: zero and NaN give a signed
-// zero, magnitudes from half a step above the largest finite value saturate to
-// it, below the smallest normal the value is a count of subnormal steps rounded
-// half up, else round to nearest even on the FP32 mantissa with the carry going
-// into the exponent.
-template <bool kE5M2>
-__device__ __forceinline__ uint32_t fp8_encode(float f) {
-    constexpr int kMant = kE5M2 ? 2 : 3, kBias = kE5M2 ? 15 : 7, kDrop = 23 - kMant;
-    constexpr uint32_t kMaxCode = kE5M2 ? 0x7Bu : 0x7Eu;
-    const uint32_t b = __builtin_bit_cast(uint32_t, f);
-    const uint32_t sign = (b >> 24) & 0x80u;
-    const float a = fabsf(f);
-    if (!(a > 0.0f)) return sign;
-    if (a >= (kE5M2 ? 61440.0f : 464.0f)) return sign | kMaxCode;
-    int e = (int)((b >> 23) & 0xFFu) - 127;
-    if (e < 1 - kBias) {
-        int q = (int)(a * (kE5M2 ? 65536.0f : 512.0f) + 0.5f);
-        q = min(q, 1 << kMant);                       // rolls into the smallest normal
-        return sign | (uint32_t)q;
-    }
-    const uint32_t m = b & 0x7FFFFFu;
-    uint32_t mm = m >> kDrop;
-    const uint32_t rem = m & ((1u << kDrop) - 1u), half_way = 1u << (kDrop - 1);
-    if (rem > half_way || (rem == half_way && (mm & 1u))) {
-        if (++mm == (1u << kMant)) { mm = 0; ++e; }
-    }
-    if (e > (kE5M2 ? 15 : 8)) return sign | kMaxCode;
-    return sign | ((uint32_t)(e + kBias) << kMant) | mm;
-}
-
 // Per head and channel the FP32 mean of the run's keys, positions in order.
 __global__ void kv_build_ref(const h16* __restrict__ k, h16* __restrict__ ref, int n_kv_heads, int n_pos) {
     const int h = (int)blockIdx.x, d = (int)threadIdx.x;

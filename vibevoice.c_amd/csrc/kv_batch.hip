@@ -1,0 +1,366 @@
+// The cache side of a serving step: many sequences that share one pool of 64-position pages.
+//
+//   page_plan       which pages and slots a step's new positions take, from the sequences' lengths.
+//   append_rows     bias, rotary embedding and the append of a step's rows, each at its own position and slot.
+//
+// Both are described at their kernels; the attention that reads the pool is in attention_batch.hip.
+#include "attn_common.hpp"
+#include "rope_common.hpp"
+
+namespace vv {
+namespace {
+
+// ── pages and slots from lengths ─────────────────────────────────────────
+// Sequence i holds len_i positions and asks for new_i more: need_i = ceil((len_i + new_i) / 64) - ceil(len_i / 64)
+// pages. Sequences are served in order: with E_i the running sum of new rows and C_i that of needed pages (both
+// through i), i is served when its positions fit its table, its rows end within max_rows (E_i <= max_rows) and it
+// needs no page or C_i <= n_free. C counts a sequence that is turned away for want of pages too, so none that needs
+// a page overtakes it, and the served ones' pages are the first C of the stack, without holes:
+// page j handed out is free[n_free - 1 - j].
+// Everything a row writes follows from its own sequence's E, C and length, so every workgroup scans the lengths for
+// itself (8 bytes a sequence, out of L2) and fills its own run of rows: one launch, no exchange between workgroups,
+// no atomics on memory. A new page's first position is always a new row, so that row writes the table entry.
+// Sums are 32 bits, held at 2^31 - 1: past that no row or page is handed out, and the saturating sum of
+// non-negative values does not depend on its grouping.
+struct PlanArgs {
+    const int* new_lens;
+    const int* cache_lens;
+    int* tables;
+    const int* free_pages;
+    const int* n_free;
+    int* lens_out;
+    int* row_starts;
+    int* positions;
+    int64_t* slots;
+    int* counts;
+    int n_seqs, max_pages, max_rows, rows_per_wg;
+};
+
+constexpr int kPlanThreads = 1024;
+
+__device__ __forceinline__ int add_capped(int a, int b) {
+    const uint32_t s = (uint32_t)a + (uint32_t)b;
+    return s > 0x7fffffffu ? 0x7fffffff : (int)s;
+}
+
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int scan_step(int v) {
+    return add_capped(v, __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xF, false));
+}
+// Inclusive sum over the wave's lanes, inside the vector ALU: shifts by 1, 2, 4, 8 within rows of 16 lanes, then the
+// last lane of a row into the next row, then of the first half into the second.
+__device__ __forceinline__ int wave_scan(int v) {
+    v = scan_step<0x111, 0xF>(v);
+    v = scan_step<0x112, 0xF>(v);
+    v = scan_step<0x114, 0xF>(v);
+    v = scan_step<0x118, 0xF>(v);
+    v = scan_step<0x142, 0xA>(v);
+    return scan_step<0x143, 0xC>(v);
+}
+// Inclusive sum over the workgroup and, in `total`, the sum of all; `sums` (an int per wave) is free again after the
+// caller's next barrier.
+__device__ __forceinline__ int block_scan(int v, int* sums, int& total) {
+    const int incl = wave_scan(v);
+    const int wave = wave_in_block(), waves = (int)blockDim.x >> 6;
+    if (lane_id() == 63) sums[wave] = incl;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+    for (int w = 0; w < waves; ++w) {
+        if (w == wave) before = total;
+        total = add_capped(total, sums[w]);
+    }
+    return add_capped(before, incl);
+}
+
+__device__ __forceinline__ int pages_of(int len) { return (int)(((unsigned)len + (kPage - 1)) / kPage); }
+
+__global__ __launch_bounds__(kPlanThreads) void page_plan(PlanArgs a) {
+    __shared__ int s_rows[kPlanThreads / kWave], s_pages[kPlanThreads / kWave];
+    __shared__ int s_end[kPlanThreads], s_start[kPlanThreads], s_len[kPlanThreads], s_fresh[kPlanThreads];
+    __shared__ int s_taken, s_refused;
+    const int tid = (int)threadIdx.x, threads = (int)blockDim.x;
+    const bool lead = blockIdx.x == 0;           // writes what there is one of: the lengths, row starts and counts
+    const int row0 = (int)min((int64_t)blockIdx.x * a.rows_per_wg, (int64_t)a.max_rows);
+    const int row1 = (int)min((int64_t)row0 + a.rows_per_wg, (int64_t)a.max_rows);
+    const int n_free = max(*a.n_free, 0);
+    if (tid == 0) { s_taken = 0; s_refused = 0; }
+
+    int rows_before = 0, pages_before = 0;
+    for (int c0 = 0; c0 < a.n_seqs; c0 += threads) {
+        const int i = c0 + tid;
+        const int asked = i < a.n_seqs ? max(a.new_lens[i], 0) : 0;
+        const int len = i < a.n_seqs ? a.cache_lens[i] : 0;
+        int rows_here, pages_here;
+        const int end = add_capped(rows_before, block_scan(asked, s_rows, rows_here));
+        const bool fits = asked > 0 && len >= 0 && (int64_t)len + asked <= (int64_t)a.max_pages * kPage &&
+                          end <= a.max_rows;
+        const int need = fits ? pages_of(len + asked) - pages_of(len) : 0;
+        const int taken = add_capped(pages_before, block_scan(need, s_pages, pages_here));
+        const bool served = fits && (need == 0 || taken <= n_free);
+        s_end[tid] = end;
+        s_start[tid] = end - asked;
+        s_len[tid] = served ? len : -1;
+        s_fresh[tid] = taken - need;
+        if (lead && i < a.n_seqs) {
+            a.lens_out[i] = len + (served ? asked : 0);
+            a.row_starts[i + 1] = min(end, a.max_rows);
+            if (served && need > 0) atomicMax(&s_taken, taken);
+            if (asked > 0 && !served) atomicAdd(&s_refused, 1);
+        }
+        __syncthreads();
+        const int rows_after = add_capped(rows_before, rows_here);
+        // Unsigned: a saturated sum plus a thread's number stays below 2^32.
+        for (unsigned r = (unsigned)max(row0, rows_before) + tid; r < (unsigned)min(row1, rows_after); r += threads) {
+            int lo = 0, hi = threads - 1;        // the first sequence of this run that ends past row r
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (s_end[mid] > (int)r) hi = mid;
+                else lo = mid + 1;
+            }
+            const int held = s_len[lo];
+            int position = 0;
+            int64_t slot = -1;
+            if (held >= 0) {
+                position = held + ((int)r - s_start[lo]);
+                const int index = position / kPage, had = pages_of(held);
+                int* entry = a.tables + (size_t)(c0 + lo) * a.max_pages + index;
+                int page;
+                if (index < had) {
+                    page = *entry;
+                } else {
+                    page = a.free_pages[n_free - 1 - (s_fresh[lo] + index - had)];
+                    if (position % kPage == 0) *entry = page;
+                }
+                if (page >= 0) slot = (int64_t)page * kPage + position % kPage;
+            }
+            a.positions[r] = position;
+            a.slots[r] = slot;
+        }
+        rows_before = rows_after;
+        pages_before = add_capped(pages_before, pages_here);
+        __syncthreads();
+        if (!lead && rows_before >= row1) return;      // the same for the whole workgroup
+    }
+    for (unsigned r = (unsigned)max(row0, rows_before) + tid; r < (unsigned)row1; r += threads) {      // rows past the last
+        a.positions[r] = 0;
+        a.slots[r] = -1;
+    }
+    if (lead && tid == 0) {
+        a.row_starts[0] = 0;
+        a.counts[0] = n_free - s_taken;
+        a.counts[1] = min(rows_before, a.max_rows);
+        a.counts[2] = s_refused;
+    }
+}
+
+// ── bias, rotation and append ────────────────────────────────────────────
+// Row r: q_out[r] = rope(q[r] + bq), K[slot_r] = rope(k[r] + bk), V[slot_r] = v[r] + bv at position pos_r; every step
+// rounds to FP16 where separate calls would store, so the bits are those of vv_bias_rope_qk_dev, vv_bias_add_dev and
+// vv_kv_store_dev on that row. A row moves 4 hd (nq + nkv) + 2 hd nkv (1 + bytes per stored value) bytes and does
+// three flops a value: bound by memory, or by its latency when there are few rows.
+// A lane's item is one pair of chunks (c, c + hd/16) of one head: the eight rotary pairs (d, d + hd/2), or for V just
+// sixteen values. Heads are counted q, then k, then v. A row takes `waves` waves; each computes the row's hd/2
+// cosines and sines, one pair per lane, and collects the eight a lane needs by lane exchange - no LDS, no barrier.
+struct AppendArgs {
+    const h16* q;
+    const h16* k;
+    const h16* v;
+    const h16* q_bias;
+    const h16* k_bias;
+    const h16* v_bias;
+    const int* positions;
+    const int64_t* slots;
+    h16* q_out;
+    void* k_store;
+    void* v_store;
+    int64_t n_slots;
+    int rows, nq, nkv, head_dim;
+};
+
+template <int kFmt>
+__device__ __forceinline__ void store_values(void* store, size_t at, const Chunk& c) {      // eight, at element `at`
+    if constexpr (kFmt == kFmtFp16) {
+        store_chunk(reinterpret_cast<Chunk*>(static_cast<h16*>(store) + at), c);
+    } else {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        const h16x8 h = __builtin_bit_cast(h16x8, c);
+        u32x2 w = {0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i >> 2] |= fp8_encode<kFmt == kFmtE5M2>((float)h[i]) << (8 * (i & 3));
+        *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(store) + at) = w;
+    }
+}
+
+template <int kHd, int kFmt>
+__global__ __launch_bounds__(kBlock) void append_rows(AppendArgs a, FreqTable freqs, int waves) {
+    constexpr int kItems = kHd / 16;              // items per head
+    constexpr int kHeads = kWave / kItems;        // heads a wave takes at a time
+    const int unit = (int)blockIdx.x * kWavesPerBlock + wave_in_block();
+    const int row = unit / waves, part = unit - row * waves;
+    if (row >= a.rows) return;                    // whole waves leave; nothing below synchronises
+    const int64_t slot = a.slots[row];
+    if (slot < 0 || slot >= a.n_slots) return;
+    const int lane = lane_id(), c = lane % kItems;
+    const int heads = a.nq + 2 * a.nkv;
+
+    float my_s, my_c;
+    sincosf((float)a.positions[row] * freqs.f[lane % (kHd / 2)], &my_s, &my_c);
+    f32x8 cv, sv;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        cv[i] = __shfl(my_c, 8 * c + i);
+        sv[i] = __shfl(my_s, 8 * c + i);
+    }
+    for (int head = part * kHeads + lane / kItems; head < heads; head += waves * kHeads) {
+        const int kind = head < a.nq ? 0 : head < a.nq + a.nkv ? 1 : 2;
+        const int h = kind == 0 ? head : kind == 1 ? head - a.nq : head - a.nq - a.nkv;
+        const h16* src = kind == 0 ? a.q + (size_t)row * a.nq * kHd
+                                   : (kind == 1 ? a.k : a.v) + (size_t)row * a.nkv * kHd;
+        const h16* bias = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
+        const Chunk* p = reinterpret_cast<const Chunk*>(src + h * kHd) + c;
+        Chunk lo = load_chunk(p), hi = load_chunk(p + kItems);
+        if (bias) {
+            const Chunk* bp = reinterpret_cast<const Chunk*>(bias + h * kHd) + c;
+            lo = add_bias(lo, load_chunk(bp));
+            hi = add_bias(hi, load_chunk(bp + kItems));
+        }
+        if (kind != 2) {
+            const f32x8 x0 = unpack(lo), x1 = unpack(hi);
+            f32x8 y0, y1;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const Pair r = rotate(x0[i], x1[i], cv[i], sv[i]);
+                y0[i] = r.lo;
+                y1[i] = r.hi;
+            }
+            lo = pack(y0);
+            hi = pack(y1);
+        }
+        if (kind == 0) {
+            Chunk* dst = reinterpret_cast<Chunk*>(a.q_out + ((size_t)row * a.nq + h) * kHd) + c;
+            store_chunk(dst, lo);
+            store_chunk(dst + kItems, hi);
+        } else {
+            void* store = kind == 1 ? a.k_store : a.v_store;
+            const size_t at = ((size_t)slot * a.nkv + h) * kHd + 8 * c;
+            store_values<kFmt>(store, at, lo);
+            store_values<kFmt>(store, at + kHd / 2, hi);
+        }
+    }
+}
+
+// Any even head_dim <= 256, any alignment, FP16 pools: a workgroup per row, 2-byte accesses.
+__global__ __launch_bounds__(kBlock) void append_generic(AppendArgs a, FreqTable freqs) {
+    __shared__ float cs_cos[kMaxPairs];
+    __shared__ float cs_sin[kMaxPairs];
+    const int half = a.head_dim / 2;
+    const size_t row = blockIdx.x;
+    const int64_t slot = a.slots[row];
+    if (slot < 0 || slot >= a.n_slots) return;
+    const int pos = a.positions[row];
+    for (int i = (int)threadIdx.x; i < half; i += kBlock) {
+        float s, c;
+        sincosf((float)pos * freqs.f[i], &s, &c);
+        cs_cos[i] = c;
+        cs_sin[i] = s;
+    }
+    __syncthreads();
+    const int tasks = (a.nq + 2 * a.nkv) * half;
+    for (int t = (int)threadIdx.x; t < tasks; t += kBlock) {
+        const int head = t / half, i = t - head * half;
+        const int kind = head < a.nq ? 0 : head < a.nq + a.nkv ? 1 : 2;
+        const int h = kind == 0 ? head : kind == 1 ? head - a.nq : head - a.nq - a.nkv;
+        const size_t in = (row * (size_t)(kind == 0 ? a.nq : a.nkv) + (size_t)h) * (size_t)a.head_dim;
+        const h16* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + in;
+        const h16* bias = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
+        h16 h0 = src[i], h1 = src[i + half];
+        if (bias) {
+            h0 = to_half((float)h0 + (float)bias[(size_t)h * a.head_dim + i]);
+            h1 = to_half((float)h1 + (float)bias[(size_t)h * a.head_dim + i + half]);
+        }
+        if (kind != 2) {
+            const Pair r = rotate((float)h0, (float)h1, cs_cos[i], cs_sin[i]);
+            h0 = to_half(r.lo);
+            h1 = to_half(r.hi);
+        }
+        h16* dst = kind == 0 ? a.q_out + in
+                             : static_cast<h16*>(kind == 1 ? a.k_store : a.v_store) +
+                                   ((size_t)slot * a.nkv + (size_t)h) * (size_t)a.head_dim;
+        dst[i] = h0;
+        dst[i + half] = h1;
+    }
+}
+
+inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+
+}  // namespace
+}  // namespace vv
+
+extern "C" {
+
+vv_status_t vv_kv_page_plan_dev(const int* new_lens, const int* cache_lens, int n_seqs, int* page_tables,
+                                int max_pages, const int* free_pages, const int* n_free, int* lens_out,
+                                int* row_starts, int* positions, int64_t* slots, int max_rows, int* counts,
+                                void* stream) {
+    if (n_seqs <= 0) return VV_OK;
+    if (!new_lens || !cache_lens || !page_tables || !free_pages || !n_free || !lens_out || !row_starts || !counts)
+        return VV_ERR_NULL_PTR;
+    if (max_pages <= 0 || max_rows < 0) return VV_ERR_INVALID_ARG;
+    if (max_rows > 0 && (!positions || !slots)) return VV_ERR_NULL_PTR;
+    if (lens_out == new_lens) return VV_ERR_INVALID_ARG;
+    vv::PlanArgs a = {new_lens, cache_lens, page_tables, free_pages, n_free, lens_out, row_starts, positions, slots,
+                      counts, n_seqs, max_pages, max_rows, max_rows};
+    const int threads = n_seqs <= 64 && max_rows <= 64 ? 64 : n_seqs <= 256 ? 256 : vv::kPlanThreads;
+    // In place the lengths (or the free count) that a workgroup still has to read are what another writes: one
+    // workgroup then, which reads before it writes.
+    const bool in_place = lens_out == cache_lens || counts == n_free;
+    if (!in_place && max_rows > threads) a.rows_per_wg = threads;
+    const unsigned wgs = a.rows_per_wg > 0 ? (unsigned)((max_rows - 1) / a.rows_per_wg + 1) : 1u;
+    vv::page_plan<<<dim3(wgs), (unsigned)threads, 0, vv::as_stream(stream)>>>(a);
+    return vv::launch_status();
+}
+
+vv_status_t vv_rope_kv_append_dev(const void* q, const void* k, const void* v, const void* q_bias,
+                                  const void* k_bias, const void* v_bias, const int* positions,
+                                  const int64_t* slots, void* q_out, void* k_store, void* v_store, int n_rows,
+                                  int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int kv_format,
+                                  float theta, void* stream) {
+    if (n_rows <= 0) return VV_OK;
+    if (!q || !k || !v || !positions || !slots || !q_out || !k_store || !v_store) return VV_ERR_NULL_PTR;
+    if (n_q_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || n_pages <= 0) return VV_ERR_INVALID_ARG;
+    if ((head_dim & 1) || head_dim > 2 * vv::kMaxPairs) return VV_ERR_UNSUPPORTED;
+    const bool fp8 = kv_format == vv::kFmtE4M3 || kv_format == vv::kFmtE5M2;
+    if (kv_format != vv::kFmtFp16 && !(fp8 && head_dim == 128)) return VV_ERR_UNSUPPORTED;
+    if ((int64_t)n_q_heads + 2 * (int64_t)n_kv_heads > (1 << 20)) return VV_ERR_UNSUPPORTED;
+    const vv::AppendArgs a = {static_cast<const vv::h16*>(q), static_cast<const vv::h16*>(k),
+                              static_cast<const vv::h16*>(v), static_cast<const vv::h16*>(q_bias),
+                              static_cast<const vv::h16*>(k_bias), static_cast<const vv::h16*>(v_bias), positions,
+                              slots, static_cast<vv::h16*>(q_out), k_store, v_store,
+                              (int64_t)n_pages * vv::kPage, n_rows, n_q_heads, n_kv_heads, head_dim};
+    const vv::FreqTable& freqs = vv::host_freqs(theta, head_dim);
+    hipStream_t st = vv::as_stream(stream);
+    const bool chunks = vv::aligned16(q) && vv::aligned16(k) && vv::aligned16(v) && vv::aligned16(q_out) &&
+                        vv::aligned16(q_bias) && vv::aligned16(k_bias) && vv::aligned16(v_bias) &&
+                        (fp8 ? vv::aligned8(k_store) && vv::aligned8(v_store)
+                             : vv::aligned16(k_store) && vv::aligned16(v_store));
+    if (fp8 && !chunks) return VV_ERR_UNSUPPORTED;
+    if (chunks && (head_dim == 128 || head_dim == 64)) {
+        const int waves = 1;
+        const int64_t wgs = ((int64_t)n_rows * waves + vv::kWavesPerBlock - 1) / vv::kWavesPerBlock;
+        const dim3 grid((unsigned)wgs);
+        if (head_dim == 64)
+            vv::append_rows<64, vv::kFmtFp16><<<grid, vv::kBlock, 0, st>>>(a, freqs, waves);
+        else if (!fp8)
+            vv::append_rows<128, vv::kFmtFp16><<<grid, vv::kBlock, 0, st>>>(a, freqs, waves);
+        else if (kv_format == vv::kFmtE4M3)
+            vv::append_rows<128, vv::kFmtE4M3><<<grid, vv::kBlock, 0, st>>>(a, freqs, waves);
+        else
+            vv::append_rows<128, vv::kFmtE5M2><<<grid, vv::kBlock, 0, st>>>(a, freqs, waves);
+    } else {
+        vv::append_generic<<<dim3((unsigned)n_rows), vv::kBlock, 0, st>>>(a, freqs);
+    }
+    return vv::launch_status();
+}
+
+}  // extern "C"

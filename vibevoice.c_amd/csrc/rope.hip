@@ -18,19 +18,12 @@
 //     value is bit-identical to what the CPU kernels compute. The device then
 //     forms the angle with one FP32 multiply and calls the full-range sincosf
 //     (never the fast intrinsics, whose error grows with |angle|).
-#include <math.h>
-
-#include "row_math.hpp"
+#include "rope_common.hpp"
 
 namespace vv {
 namespace {
 
-constexpr int kMaxPairs = 128;      // head_dim <= 256
 constexpr int kPosPerBlock = 4;     // positions per workgroup in the head_dim-128 kernel
-
-struct FreqTable {
-    float f[kMaxPairs];
-};
 
 struct RopeArgs {
     h16* q;                 // [rows, nq, head_dim] or nullptr
@@ -40,14 +33,6 @@ struct RopeArgs {
     const int* d_position;  // device int with the first row's position, or nullptr
     int rows, nq, nk, head_dim, position_offset;
 };
-
-__device__ __forceinline__ Chunk add_bias(const Chunk& v, const Chunk& b) {
-    const f32x8 x = unpack(v), y = unpack(b);
-    f32x8 r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = x[i] + y[i];
-    return pack(r);      // rounded to FP16 before the rotation, as bias_add then rope would
-}
 
 // head_dim == 128, 16-byte aligned tensors, at most kMaxFastHeads heads in all.
 //
@@ -335,22 +320,6 @@ __global__ __launch_bounds__(kBlock) void rope128_pair_from_table(h16* __restric
     }
     store_chunk(lo_p, pack(y0));
     store_chunk(lo_p + 8, pack(y1));
-}
-
-// The table depends only on (theta, head_dim); each host thread remembers the
-// last one it built (thread-local, so concurrent callers never share state).
-const FreqTable& host_freqs(float theta, int head_dim) {
-    thread_local FreqTable table;
-    thread_local float cached_theta = 0.0f;
-    thread_local int cached_dim = 0;
-    if (cached_dim != head_dim || cached_theta != theta) {
-        const int half = head_dim / 2;
-        for (int i = 0; i < kMaxPairs; ++i)
-            table.f[i] = i < half ? powf(theta, -2.0f * (float)i / (float)head_dim) : 0.0f;
-        cached_theta = theta;
-        cached_dim = head_dim;
-    }
-    return table;
 }
 
 vv_status_t launch_rope(void* q, void* k, const void* q_bias, const void* k_bias, int rows,

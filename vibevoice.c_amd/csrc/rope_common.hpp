@@ -1,0 +1,40 @@
+// What the rotary kernels share: the frequency table that a launch carries in its arguments, and the projection bias.
+#pragma once
+
+#include <math.h>
+
+#include "row_math.hpp"
+
+namespace vv {
+
+constexpr int kMaxPairs = 128;      // head_dim <= 256
+
+struct FreqTable {
+    float f[kMaxPairs];
+};
+
+__device__ __forceinline__ Chunk add_bias(const Chunk& v, const Chunk& b) {
+    const f32x8 x = unpack(v), y = unpack(b);
+    f32x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i] + y[i];
+    return pack(r);      // rounded to FP16 before the rotation, as bias_add then rope would
+}
+
+// The table depends only on (theta, head_dim); each host thread remembers the
+// last one it built (thread-local, so concurrent callers never share state).
+inline const FreqTable& host_freqs(float theta, int head_dim) {
+    thread_local FreqTable table;
+    thread_local float cached_theta = 0.0f;
+    thread_local int cached_dim = 0;
+    if (cached_dim != head_dim || cached_theta != theta) {
+        const int half = head_dim / 2;
+        for (int i = 0; i < kMaxPairs; ++i)
+            table.f[i] = i < half ? powf(theta, -2.0f * (float)i / (float)head_dim) : 0.0f;
+        cached_theta = theta;
+        cached_dim = head_dim;
+    }
+    return table;
+}
+
+}  // namespace vv
