@@ -660,22 +660,25 @@ vv_status_t vv_kv_page_map_dev(int* page_table, int first, int n, const int* pag
  *   row_starts[n_seqs + 1] first packed row of each sequence: the running sum of new_lens (refused ones included, so
  *                          rows keep the places the caller packed them in), held at max_rows
  *   positions, slots [max_rows]  of each packed row; 0 and -1 for rows of refused sequences and rows past the last
- *   counts[3]              free pages left, rows in use (row_starts[n_seqs]), sequences refused
- * free_pages is not written: the pages in use are its top counts-many, so the caller carries counts[0] as the next
- * *n_free, and returns a finished sequence's pages by writing them back from free_pages[*n_free] on.
- * lens_out may be cache_lens and counts may be n_free (a captured step that advances itself); one workgroup then fills
- * all rows. lens_out == new_lens: VV_ERR_INVALID_ARG. Replaces vv_kv_page_map_dev and host-side slot arithmetic
- * per sequence. */
+ *   n_free_out             free pages left on the stack, the next step's *n_free; may be NULL
+ *   counts[3]              the balance of pages: *n_free less all that were asked for up to the last sequence served
+ *                          (equal to *n_free_out unless a sequence before that was refused for want of pages; below
+ *                          zero by what was missing), rows in use (row_starts[n_seqs]), sequences refused
+ * free_pages is not written: a finished sequence's pages return by being written from free_pages[*n_free] on.
+ * lens_out may be cache_lens and n_free_out may be n_free (a captured step that advances itself); one workgroup then
+ * fills all rows. Other overlaps are the caller's mistake; lens_out == new_lens and counts == n_free are refused with
+ * VV_ERR_INVALID_ARG. Takes the place of vv_kv_page_map_dev and of the host's slot arithmetic per sequence. */
 vv_status_t vv_kv_page_plan_dev(const int* new_lens, const int* cache_lens, int n_seqs, int* page_tables,
                                 int max_pages, const int* free_pages, const int* n_free, int* lens_out,
-                                int* row_starts, int* positions, int64_t* slots, int max_rows, int* counts,
-                                void* stream);
+                                int* row_starts, int* positions, int64_t* slots, int max_rows, int* n_free_out,
+                                int* counts, void* stream);
 
 /* addition: bias, rotary embedding and KV append of n_rows packed rows, each at its own position and slot (what
  * vv_kv_page_plan_dev writes): q_out[r] = rope(q[r] + q_bias, positions[r]) (q_out may be q), and, into row slots[r] of
  * the pool, rope(k[r] + k_bias, positions[r]) and v[r] + v_bias. q, q_out [n_rows][n_q_heads][head_dim], k, v
- * [n_rows][n_kv_heads][head_dim] FP16; a bias may be NULL. Every step rounds to FP16 where the separate calls store:
- * the bits are those of vv_bias_add_dev, vv_rope_qk_dev and vv_kv_store_dev (without a reference key) on each row.
+ * [n_rows][n_kv_heads][head_dim] FP16; a bias may be NULL. FP32 arithmetic and one rounding to FP16, of which an FP8
+ * pool takes the code: without biases the bits are those of vv_rope_qk_dev and vv_kv_store_dev (without a reference
+ * key) on each row; with them q and K are spared the rounding that vv_bias_add_dev does before the rotation.
  * A row whose slot is negative or not below 64 * n_pages is skipped: nothing of it is read or written, q_out
  * included. Slots must differ from one another; of two rows with one slot either may win, vector piece by piece.
  * kv_format FP16: any even head_dim <= 256 and 2-byte alignment (head_dim 64 and 128 with everything 16-byte aligned

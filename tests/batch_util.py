@@ -15,7 +15,7 @@ def plan(new_lens, cache_lens, tables, free, n_free, max_rows):
     tables = tables.copy()
     starts, lens = [0], list(cache_lens)
     positions, slots = np.zeros(max_rows, np.int32), np.full(max_rows, -1, np.int64)
-    asked_pages = taken = refused = 0
+    asked_pages = taken = refused = asked_by_served = 0
     n_free = max(n_free, 0)
     for i in range(n):
         new, held = max(int(new_lens[i]), 0), int(cache_lens[i])
@@ -34,6 +34,7 @@ def plan(new_lens, cache_lens, tables, free, n_free, max_rows):
         for j in range(need):
             tables[i, pages_of(held) + j] = free[n_free - 1 - taken - j]
         taken += need
+        asked_by_served = asked_pages
         lens[i] = held + new
         for r in range(new):
             p = held + r
@@ -42,7 +43,8 @@ def plan(new_lens, cache_lens, tables, free, n_free, max_rows):
             slots[begin + r] = page * PAGE + p % PAGE if page >= 0 else -1
     starts = np.minimum(np.array(starts, np.int64), max_rows).astype(np.int32)
     return {"tables": tables, "lens": np.array(lens, np.int32), "row_starts": starts, "positions": positions,
-            "slots": slots, "counts": np.array([n_free - taken, starts[-1], refused], np.int32)}
+            "slots": slots, "n_free": n_free - taken,
+            "counts": np.array([n_free - asked_by_served, starts[-1], refused], np.int32)}
 
 
 def slots_of(table_row, length):

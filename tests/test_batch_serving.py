@@ -14,7 +14,8 @@ P = 0x1000      # a non-null, 16-byte aligned stand-in; never dereferenced by th
 
 def plan_call(**change):
     a = dict(new_lens=P, cache_lens=P + 64, n_seqs=4, tables=P, max_pages=8, free=P, n_free=P, lens_out=P + 128,
-             row_starts=P, positions=P, slots=P, max_rows=16, counts=P + 256, stream=None)
+             row_starts=P, positions=P, slots=P, max_rows=16, n_free_out=P + 192, counts=P + 256,
+             stream=None)
     a.update(change)
     return dev.vv_kv_page_plan_dev(*a.values())
 
@@ -48,6 +49,7 @@ def test_plan_refusals():
     assert plan_call(max_pages=0) == dev.VV_ERR_INVALID_ARG
     assert plan_call(max_rows=-1) == dev.VV_ERR_INVALID_ARG
     assert plan_call(lens_out=P) == dev.VV_ERR_INVALID_ARG            # the lengths over the request they follow from
+    assert plan_call(counts=P) == dev.VV_ERR_INVALID_ARG              # the counts over the number of free pages
 
 
 @pytest.mark.parametrize("name", ["q", "k", "v", "positions", "slots", "q_out", "k_store", "v_store"])
@@ -110,6 +112,7 @@ def test_the_plain_plan_hands_out_pages_like_a_stack():
     got = plan([1, 65, 1], [64, 0, 127], tables, [20, 21, 22, 23], 4, 70)
     assert got["tables"].tolist() == [[5, 23, -1], [22, 21, -1], [7, 8, -1]]
     assert got["lens"].tolist() == [65, 65, 128] and got["counts"].tolist() == [1, 67, 0]
+    assert got["n_free"] == 1
     assert got["row_starts"].tolist() == [0, 1, 66, 67]
     assert got["slots"][0] == 23 * PAGE and got["slots"][1] == 22 * PAGE and got["slots"][65] == 21 * PAGE
     assert got["slots"][66] == 8 * PAGE + 63 and (got["slots"][67:] == -1).all()
@@ -118,6 +121,7 @@ def test_the_plain_plan_hands_out_pages_like_a_stack():
     # too few pages: the second is refused, and the third, which needs one, does not overtake it; the fourth needs none
     tables = np.array([[5, -1], [-1, -1], [6, -1], [7, -1]], np.int32)
     got = plan([1, 128, 1, 1], [64, 0, 64, 3], tables, [20, 21], 2, 200)
-    assert got["lens"].tolist() == [65, 0, 64, 4] and got["counts"].tolist() == [1, 131, 2]
+    assert got["lens"].tolist() == [65, 0, 64, 4] and got["n_free"] == 1
+    assert got["counts"].tolist() == [-2, 131, 2]        # 2 less the 1 + 2 + 1 asked for up to the last one served
     assert (got["slots"][1:130] == -1).all() and got["slots"][130] == 7 * PAGE + 3
     assert pages_of(0) == 0 and pages_of(1) == 1 and pages_of(64) == 1 and pages_of(65) == 2

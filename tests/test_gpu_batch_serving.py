@@ -28,8 +28,8 @@ def run_plan(new, lens, tables, free, n_free, max_rows, in_place=False, pad=7):
     n, max_pages = tables.shape
     d = dict(new=ints(new), lens=ints(lens), tables=ints(tables), free=ints(free if len(free) else [0]),
              counts=torch.full((3,), -77, dtype=torch.int32, device="cuda"))
-    d["counts"][0] = n_free
-    d["n_free"] = d["counts"] if in_place else ints([n_free])
+    d["n_free"] = ints([n_free])
+    d["n_free_out"] = d["n_free"] if in_place else ints([-77])
     d["lens_out"] = d["lens"] if in_place else torch.full((n,), -77, dtype=torch.int32, device="cuda")
     d["starts"] = torch.full((n + 1 + pad,), -77, dtype=torch.int32, device="cuda")
     d["positions"] = torch.full((max_rows + pad,), -77, dtype=torch.int32, device="cuda")
@@ -37,13 +37,14 @@ def run_plan(new, lens, tables, free, n_free, max_rows, in_place=False, pad=7):
     ok(dev.vv_kv_page_plan_dev(d["new"].data_ptr(), d["lens"].data_ptr(), n, d["tables"].data_ptr(), max_pages,
                                d["free"].data_ptr(), d["n_free"].data_ptr(), d["lens_out"].data_ptr(),
                                d["starts"].data_ptr(), d["positions"].data_ptr(), d["slots"].data_ptr(), max_rows,
-                               d["counts"].data_ptr(), stream()))
+                               d["n_free_out"].data_ptr(), d["counts"].data_ptr(), stream()))
     torch.cuda.synchronize()
     assert (d["starts"][n + 1:] == -77).all() and (d["positions"][max_rows:] == -77).all() and \
         (d["slots"][max_rows:] == -77).all(), "written past the end"
     return {"tables": d["tables"].cpu().numpy(), "lens": d["lens_out"].cpu().numpy(),
             "row_starts": d["starts"][:n + 1].cpu().numpy(), "positions": d["positions"][:max_rows].cpu().numpy(),
-            "slots": d["slots"][:max_rows].cpu().numpy(), "counts": d["counts"].cpu().numpy()}
+            "slots": d["slots"][:max_rows].cpu().numpy(), "counts": d["counts"].cpu().numpy(),
+            "n_free": int(d["n_free_out"])}
 
 
 def check_plan(new, lens, max_pages, n_free, max_rows, seed, in_place=False):
@@ -80,7 +81,7 @@ def test_plan(n, top, chunk, rows, free, in_place):
 def test_plan_refuses_one_at_a_time():
     # refused: a negative length, 120 + 10 > 128 positions, 0 + 200 > 128; a negative request asks for nothing
     want = check_plan([2, 1, -5, 10, 200, 3, 1], [63, -1, 5, 120, 0, 1, 64], 2, 3, 300, 1)
-    assert want["counts"].tolist() == [1, 217, 3] and want["lens"].tolist() == [65, -1, 5, 120, 0, 4, 65]
+    assert want["counts"].tolist() == [1, 217, 3] and want["n_free"] == 1 and want["lens"].tolist() == [65, -1, 5, 120, 0, 4, 65]
     check_plan([0, 0, 0], [5, 0, 64], 2, 0, 4, 2)                       # nothing asked
     check_plan([1, 1], [5, 7], 1, 0, 0, 3)                              # no rows at all
     check_plan([1, 1], [64, 7], 2, -4, 3, 4)                            # a pool that is overdrawn already
@@ -100,7 +101,8 @@ def test_plan_captured_advances_itself():
         at += pages_of(x)
     free, n_free = perm[at:], pool - at
     d_new, d_lens, d_tables, d_free = ints(np.ones(n)), ints(lens), ints(tables), ints(free)
-    counts, starts = ints([n_free, 0, 0]), torch.zeros(n + 1, dtype=torch.int32, device="cuda")
+    d_n_free, counts = ints([n_free]), ints([0, 0, 0])
+    starts = torch.zeros(n + 1, dtype=torch.int32, device="cuda")
     positions = torch.zeros(n, dtype=torch.int32, device="cuda")
     slots = torch.zeros(n, dtype=torch.int64, device="cuda")
     s = torch.cuda.Stream()
@@ -108,14 +110,16 @@ def test_plan_captured_advances_itself():
     h = C.c_void_p()
     ok(dev.vv_dev_graph_begin(s.cuda_stream))
     ok(dev.vv_kv_page_plan_dev(d_new.data_ptr(), d_lens.data_ptr(), n, d_tables.data_ptr(), max_pages,
-                               d_free.data_ptr(), counts.data_ptr(), d_lens.data_ptr(), starts.data_ptr(),
-                               positions.data_ptr(), slots.data_ptr(), n, counts.data_ptr(), s.cuda_stream))
+                               d_free.data_ptr(), d_n_free.data_ptr(), d_lens.data_ptr(), starts.data_ptr(),
+                               positions.data_ptr(), slots.data_ptr(), n, d_n_free.data_ptr(), counts.data_ptr(),
+                               s.cuda_stream))
     ok(dev.vv_dev_graph_end(s.cuda_stream, C.byref(h)))
     for _ in range(70):
         want = plan(np.ones(n, int), lens, tables, free, n_free, n)
         ok(dev.vv_dev_graph_launch(h, s.cuda_stream))
         ok(dev.vv_dev_stream_sync(s.cuda_stream))
-        lens, tables, n_free = want["lens"], want["tables"], int(want["counts"][0])
+        lens, tables, n_free = want["lens"], want["tables"], want["n_free"]
+        assert int(d_n_free) == n_free
         assert np.array_equal(d_lens.cpu().numpy(), lens) and np.array_equal(d_tables.cpu().numpy(), tables)
         assert np.array_equal(slots.cpu().numpy(), want["slots"]) and np.array_equal(counts.cpu().numpy(),
                                                                                      want["counts"])
@@ -163,7 +167,7 @@ APPEND = [(1, 28, 4, 128, FP16), (17, 28, 4, 128, FP16), (70, 12, 2, 128, FP16),
 
 @pytest.mark.parametrize("biased", [True, False])
 @pytest.mark.parametrize("rows,nq,nkv,hd,fmt", APPEND)
-def test_append_is_the_separate_calls(rows, nq, nkv, hd, fmt, biased):
+def test_append_against_the_separate_calls(rows, nq, nkv, hd, fmt, biased):
     n_pages, seed = pages_of(rows) + 2, rows * nq
     rng = np.random.default_rng(seed)
     q, k, v = (to_dev(oracle.normal_f16((rows, n, hd), seed + i, std=2.0)) for i, n in enumerate((nq, nkv, nkv)))
@@ -187,14 +191,37 @@ def test_append_is_the_separate_calls(rows, nq, nkv, hd, fmt, biased):
 
     out = torch.full_like(q, float("nan"))
     call(out)
-    assert np.array_equal(raw(out), raw(want_q)), "q"
-    assert np.array_equal(raw(ks), raw(want_k)) and np.array_equal(raw(vs), raw(want_v)), "pool"
+    assert np.array_equal(raw(vs), raw(want_v)), "values"
+    live = (slots >= 0) & (slots < n_pages * PAGE)
+    if not any(b is not None for b in biases[:2]):
+        assert np.array_equal(raw(out), raw(want_q)) and np.array_equal(raw(ks), raw(want_k)), "q, keys"
+    else:
+        # the separate calls round x + bias to FP16 before they turn it, 2^-11 of each of a pair; then both sides round
+        # (2^-11 each, of values that differ by that much), and an FP8 pool once more
+        def pair(x, b):
+            y = x.double().abs() + (b.double().abs() if b is not None else 0.0)
+            y = y[..., :hd // 2] + y[..., hd // 2:]
+            return torch.cat([y, y], -1)
+
+        at = torch.from_numpy(slots[live]).cuda()
+        on = torch.from_numpy(np.flatnonzero(live)).cuda()
+        code = {FP16: (0.0, 0.0), E4M3: (2.0 ** -4, 2.0 ** -9), E5M2: (2.0 ** -3, 2.0 ** -16)}[fmt]
+        for got, want, mag, low in ((out[on], want_q[on], pair(q, biases[0])[on], (0.0, 0.0)),
+                                    (ks[at], want_k[at], pair(k, biases[1])[on], code)):
+            if got.dtype == torch.uint8:
+                got, want = (t.view(TORCH_FP8[fmt]).float() for t in (got, want))
+            want = want.double()
+            off = mag * 2.0 ** -11 + (want.abs() + mag * 2.0 ** -11) * 2.0 ** -10 + 2.0 ** -24
+            off = off + 2.0 * low[0] * (want.abs() + off) + low[1]
+            assert ((got.double() - want).abs() <= off).all()
+        untouched = torch.ones(ks.shape[0], dtype=torch.bool, device="cuda")
+        untouched[at] = False
+        assert np.array_equal(raw(ks[untouched]), raw(want_k[untouched])), "rows that no slot names"
     assert all(np.array_equal(raw(x), b) for x, b in zip((q, k, v), before)), "an input was written"
     # in place: the rows of skipped slots keep q as it was
     call(q)
-    live = (slots >= 0) & (slots < n_pages * PAGE)
     at = torch.from_numpy(np.flatnonzero(live)).cuda()
-    assert np.array_equal(raw(q[at]), raw(want_q[at]))
+    assert np.array_equal(raw(q[at]), raw(out[at]))
     rest = np.flatnonzero(~live)
     assert np.array_equal(raw(q)[rest], before[0][rest])
 
@@ -215,7 +242,7 @@ def test_append_against_the_formula(fmt):
     out, ks, vs = torch.zeros_like(d[0]), new_store(n_pages, nkv, hd, fmt), new_store(n_pages, nkv, hd, fmt)
     ok(dev.vv_rope_kv_append_dev(*(x.data_ptr() for x in d), d_pos.data_ptr(), d_slots.data_ptr(), out.data_ptr(),
                                  ks.data_ptr(), vs.data_ptr(), rows, nq, nkv, hd, n_pages, fmt, 1e6, stream()))
-    x = [(oracle.widen(a) + oracle.widen(b)).astype(np.float16).astype(np.float64) for a, b in zip((q, k, v), bias)]
+    x = [oracle.widen(a).astype(np.float64) + oracle.widen(b) for a, b in zip((q, k, v), bias)]
     angle = positions[:, None] * 1e6 ** (-2.0 * np.arange(hd // 2) / hd)
     angle = np.concatenate([angle, angle], -1)[:, None, :]
     half = 2.0 ** -11
@@ -247,6 +274,8 @@ def test_append_unaligned(which):
     rng = np.random.default_rng(which)
     sizes = [(rows, nq, hd), (rows, nkv, hd), (rows, nkv, hd), (nq, hd), (nkv, hd), (nkv, hd)]
     x = [to_dev(oracle.normal_f16(s, 30 + i)) for i, s in enumerate(sizes)]
+    for bias in x[3:5]:
+        bias.zero_()                                        # q and K are then the separate calls' bits
     positions, slots = rng.integers(0, 9000, rows), rng.permutation(n_pages * PAGE)[:rows]
     want = separate_calls(*x[:3], x[3:], positions, slots, n_pages, FP16)
     if which < 6:
@@ -512,7 +541,7 @@ def test_serving_loop(fmt, captured):
     nq, nkv, hd, n, max_pages, steps, theta = 8, 2, 128, 6, 3, 12, 1e4
     pool_pages, max_rows = 9, 8
     k_store, v_store = new_store(pool_pages, nkv, hd, fmt), new_store(pool_pages, nkv, hd, fmt)
-    lens, counts = torch.zeros(n, dtype=torch.int32, device="cuda"), ints([pool_pages, 0, 0])
+    lens, n_free, counts = torch.zeros(n, dtype=torch.int32, device="cuda"), ints([pool_pages]), ints([0, 0, 0])
     tables = torch.full((n, max_pages), -1, dtype=torch.int32, device="cuda")
     free = ints(np.random.default_rng(0).permutation(pool_pages))
     new = torch.ones(n, dtype=torch.int32, device="cuda")
@@ -533,8 +562,9 @@ def test_serving_loop(fmt, captured):
 
     def launch(b, rows, st):
         ok(dev.vv_kv_page_plan_dev(new.data_ptr(), lens.data_ptr(), n, tables.data_ptr(), max_pages, free.data_ptr(),
-                                   counts.data_ptr(), lens.data_ptr(), b["starts"].data_ptr(),
-                                   b["positions"].data_ptr(), b["slots"].data_ptr(), rows, counts.data_ptr(), st))
+                                   n_free.data_ptr(), lens.data_ptr(), b["starts"].data_ptr(),
+                                   b["positions"].data_ptr(), b["slots"].data_ptr(), rows, n_free.data_ptr(),
+                                   counts.data_ptr(), st))
         ok(dev.vv_rope_kv_append_dev(b["q"].data_ptr(), b["k"].data_ptr(), b["v"].data_ptr(), None, None, None,
                                      b["positions"].data_ptr(), b["slots"].data_ptr(), b["qr"].data_ptr(),
                                      k_store.data_ptr(), v_store.data_ptr(), rows, nq, nkv, hd, pool_pages, fmt, theta, st))
@@ -558,7 +588,7 @@ def test_serving_loop(fmt, captured):
 
     def expect(ask, x, rows):
         want = plan(ask, state["lens"], state["tables"], free.cpu().numpy(), state["n_free"], rows)
-        state.update(lens=want["lens"], tables=want["tables"], n_free=int(want["counts"][0]))
+        state.update(lens=want["lens"], tables=want["tables"], n_free=want["n_free"])
         turn = theta ** (-2.0 * np.arange(hd // 2) / hd)
         for i in range(n):
             for r in range(want["row_starts"][i], want["row_starts"][i + 1]):
@@ -597,7 +627,7 @@ def test_serving_loop(fmt, captured):
         torch.cuda.synchronize()
         want = expect(ask, x, max_rows)
         refused += int(want["counts"][2])
-        assert np.array_equal(counts.cpu().numpy(), want["counts"])
+        assert np.array_equal(counts.cpu().numpy(), want["counts"]) and int(n_free) == want["n_free"]
         assert np.array_equal(small["slots"].cpu().numpy(), want["slots"])
         assert np.array_equal(tables.cpu().numpy(), want["tables"]) and np.array_equal(lens.cpu().numpy(), want["lens"])
         # attention reads row i of qr for sequence i; the requests that asked nothing shift the rows, so hold the

@@ -32,6 +32,7 @@ struct PlanArgs {
     int* row_starts;
     int* positions;
     int64_t* slots;
+    int* n_free_out;         // or nullptr
     int* counts;
     int n_seqs, max_pages, max_rows, rows_per_wg;
 };
@@ -78,13 +79,13 @@ __device__ __forceinline__ int pages_of(int len) { return (int)(((unsigned)len +
 __global__ __launch_bounds__(kPlanThreads) void page_plan(PlanArgs a) {
     __shared__ int s_rows[kPlanThreads / kWave], s_pages[kPlanThreads / kWave];
     __shared__ int s_end[kPlanThreads], s_start[kPlanThreads], s_len[kPlanThreads], s_fresh[kPlanThreads];
-    __shared__ int s_taken, s_refused;
+    __shared__ int s_asked, s_given, s_refused;
     const int tid = (int)threadIdx.x, threads = (int)blockDim.x;
     const bool lead = blockIdx.x == 0;           // writes what there is one of: the lengths, row starts and counts
     const int row0 = (int)min((int64_t)blockIdx.x * a.rows_per_wg, (int64_t)a.max_rows);
     const int row1 = (int)min((int64_t)row0 + a.rows_per_wg, (int64_t)a.max_rows);
     const int n_free = max(*a.n_free, 0);
-    if (tid == 0) { s_taken = 0; s_refused = 0; }
+    if (tid == 0) { s_asked = 0; s_given = 0; s_refused = 0; }
 
     int rows_before = 0, pages_before = 0;
     for (int c0 = 0; c0 < a.n_seqs; c0 += threads) {
@@ -105,7 +106,8 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan(PlanArgs a) {
         if (lead && i < a.n_seqs) {
             a.lens_out[i] = len + (served ? asked : 0);
             a.row_starts[i + 1] = min(end, a.max_rows);
-            if (served && need > 0) atomicMax(&s_taken, taken);
+            if (served) atomicMax(&s_asked, taken);
+            if (served && need > 0) atomicMax(&s_given, taken);
             if (asked > 0 && !served) atomicAdd(&s_refused, 1);
         }
         __syncthreads();
@@ -148,16 +150,18 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan(PlanArgs a) {
     }
     if (lead && tid == 0) {
         a.row_starts[0] = 0;
-        a.counts[0] = n_free - s_taken;
+        if (a.n_free_out) *a.n_free_out = n_free - s_given;
+        a.counts[0] = n_free - s_asked;
         a.counts[1] = min(rows_before, a.max_rows);
         a.counts[2] = s_refused;
     }
 }
 
 // ── bias, rotation and append ────────────────────────────────────────────
-// Row r: q_out[r] = rope(q[r] + bq), K[slot_r] = rope(k[r] + bk), V[slot_r] = v[r] + bv at position pos_r; every step
-// rounds to FP16 where separate calls would store, so the bits are those of vv_bias_rope_qk_dev, vv_bias_add_dev and
-// vv_kv_store_dev on that row. A row moves 4 hd (nq + nkv) + 2 hd nkv (1 + bytes per stored value) bytes and does
+// Row r: q_out[r] = rope(q[r] + bq), K[slot_r] = rope(k[r] + bk), V[slot_r] = v[r] + bv at position pos_r, in FP32 with
+// one rounding to FP16 (a biased value is not rounded before it is turned: separate calls, which store it there, are
+// off by sqrt(2) as much). The angle and the rotation are those of vv_rope_dev, and an FP8 code is that of the
+// FP16 value, so without biases the bits are those of vv_rope_qk_dev and vv_kv_store_dev on that row. A row moves 4 hd (nq + nkv) + 2 hd nkv (1 + bytes per stored value) bytes and does
 // three flops a value: bound by memory, or by its latency when there are few rows.
 // A lane's item is one pair of chunks (c, c + hd/16) of one head: the eight rotary pairs (d, d + hd/2), or for V just
 // sixteen values. Heads are counted q, then k, then v. A row takes `waves` waves; each computes the row's hd/2
@@ -219,24 +223,25 @@ __global__ __launch_bounds__(kBlock) void append_rows(AppendArgs a, FreqTable fr
                                    : (kind == 1 ? a.k : a.v) + (size_t)row * a.nkv * kHd;
         const h16* bias = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
         const Chunk* p = reinterpret_cast<const Chunk*>(src + h * kHd) + c;
-        Chunk lo = load_chunk(p), hi = load_chunk(p + kItems);
+        f32x8 x0 = unpack(load_chunk(p)), x1 = unpack(load_chunk(p + kItems));
         if (bias) {
             const Chunk* bp = reinterpret_cast<const Chunk*>(bias + h * kHd) + c;
-            lo = add_bias(lo, load_chunk(bp));
-            hi = add_bias(hi, load_chunk(bp + kItems));
+            const f32x8 b0 = unpack(load_chunk(bp)), b1 = unpack(load_chunk(bp + kItems));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x0[i] += b0[i];
+                x1[i] += b1[i];
+            }
         }
         if (kind != 2) {
-            const f32x8 x0 = unpack(lo), x1 = unpack(hi);
-            f32x8 y0, y1;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const Pair r = rotate(x0[i], x1[i], cv[i], sv[i]);
-                y0[i] = r.lo;
-                y1[i] = r.hi;
+                x0[i] = r.lo;
+                x1[i] = r.hi;
             }
-            lo = pack(y0);
-            hi = pack(y1);
         }
+        const Chunk lo = pack(x0), hi = pack(x1);
         if (kind == 0) {
             Chunk* dst = reinterpret_cast<Chunk*>(a.q_out + ((size_t)row * a.nq + h) * kHd) + c;
             store_chunk(dst, lo);
@@ -274,21 +279,21 @@ __global__ __launch_bounds__(kBlock) void append_generic(AppendArgs a, FreqTable
         const size_t in = (row * (size_t)(kind == 0 ? a.nq : a.nkv) + (size_t)h) * (size_t)a.head_dim;
         const h16* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + in;
         const h16* bias = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
-        h16 h0 = src[i], h1 = src[i + half];
+        float x0 = (float)src[i], x1 = (float)src[i + half];
         if (bias) {
-            h0 = to_half((float)h0 + (float)bias[(size_t)h * a.head_dim + i]);
-            h1 = to_half((float)h1 + (float)bias[(size_t)h * a.head_dim + i + half]);
+            x0 += (float)bias[(size_t)h * a.head_dim + i];
+            x1 += (float)bias[(size_t)h * a.head_dim + i + half];
         }
         if (kind != 2) {
-            const Pair r = rotate((float)h0, (float)h1, cs_cos[i], cs_sin[i]);
-            h0 = to_half(r.lo);
-            h1 = to_half(r.hi);
+            const Pair r = rotate(x0, x1, cs_cos[i], cs_sin[i]);
+            x0 = r.lo;
+            x1 = r.hi;
         }
         h16* dst = kind == 0 ? a.q_out + in
                              : static_cast<h16*>(kind == 1 ? a.k_store : a.v_store) +
                                    ((size_t)slot * a.nkv + (size_t)h) * (size_t)a.head_dim;
-        dst[i] = h0;
-        dst[i + half] = h1;
+        dst[i] = to_half(x0);
+        dst[i + half] = to_half(x1);
     }
 }
 
@@ -301,20 +306,20 @@ extern "C" {
 
 vv_status_t vv_kv_page_plan_dev(const int* new_lens, const int* cache_lens, int n_seqs, int* page_tables,
                                 int max_pages, const int* free_pages, const int* n_free, int* lens_out,
-                                int* row_starts, int* positions, int64_t* slots, int max_rows, int* counts,
-                                void* stream) {
+                                int* row_starts, int* positions, int64_t* slots, int max_rows, int* n_free_out,
+                                int* counts, void* stream) {
     if (n_seqs <= 0) return VV_OK;
     if (!new_lens || !cache_lens || !page_tables || !free_pages || !n_free || !lens_out || !row_starts || !counts)
         return VV_ERR_NULL_PTR;
     if (max_pages <= 0 || max_rows < 0) return VV_ERR_INVALID_ARG;
     if (max_rows > 0 && (!positions || !slots)) return VV_ERR_NULL_PTR;
-    if (lens_out == new_lens) return VV_ERR_INVALID_ARG;
+    if (lens_out == new_lens || counts == n_free) return VV_ERR_INVALID_ARG;
     vv::PlanArgs a = {new_lens, cache_lens, page_tables, free_pages, n_free, lens_out, row_starts, positions, slots,
-                      counts, n_seqs, max_pages, max_rows, max_rows};
+                      n_free_out, counts, n_seqs, max_pages, max_rows, max_rows};
     const int threads = n_seqs <= 64 && max_rows <= 64 ? 64 : n_seqs <= 256 ? 256 : vv::kPlanThreads;
     // In place the lengths (or the free count) that a workgroup still has to read are what another writes: one
     // workgroup then, which reads before it writes.
-    const bool in_place = lens_out == cache_lens || counts == n_free;
+    const bool in_place = lens_out == cache_lens || n_free_out == n_free;
     if (!in_place && max_rows > threads) a.rows_per_wg = threads;
     const unsigned wgs = a.rows_per_wg > 0 ? (unsigned)((max_rows - 1) / a.rows_per_wg + 1) : 1u;
     vv::page_plan<<<dim3(wgs), (unsigned)threads, 0, vv::as_stream(stream)>>>(a);

@@ -34,6 +34,14 @@ struct RopeArgs {
     int rows, nq, nk, head_dim, position_offset;
 };
 
+__device__ __forceinline__ Chunk add_bias(const Chunk& v, const Chunk& b) {
+    const f32x8 x = unpack(v), y = unpack(b);
+    f32x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i] + y[i];
+    return pack(r);      // rounded to FP16 before the rotation, as bias_add then rope would
+}
+
 // head_dim == 128, 16-byte aligned tensors, at most kMaxFastHeads heads in all.
 //
 // A workgroup owns `posb` consecutive positions. Work item = (position, head,

@@ -1,4 +1,4 @@
-// What the rotary kernels share: the frequency table that a launch carries in its arguments, and the projection bias.
+// What the rotary kernels share: the frequency table that a launch carries in its arguments.
 #pragma once
 
 #include <math.h>
@@ -12,14 +12,6 @@ constexpr int kMaxPairs = 128;      // head_dim <= 256
 struct FreqTable {
     float f[kMaxPairs];
 };
-
-__device__ __forceinline__ Chunk add_bias(const Chunk& v, const Chunk& b) {
-    const f32x8 x = unpack(v), y = unpack(b);
-    f32x8 r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = x[i] + y[i];
-    return pack(r);      // rounded to FP16 before the rotation, as bias_add then rope would
-}
 
 // The table depends only on (theta, head_dim); each host thread remembers the
 // last one it built (thread-local, so concurrent callers never share state).

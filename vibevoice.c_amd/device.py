@@ -107,7 +107,7 @@ SIGNATURES = {
     "vv_kv_store_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_bool, _i, _i, _i, _vp, _i,
                             _i, _vp, _vp]),
     "vv_kv_page_map_dev": (_i, [_vp, _i, _i, _vp, _vp]),
-    "vv_kv_page_plan_dev": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp]),
+    "vv_kv_page_plan_dev": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp]),
     "vv_rope_kv_append_dev": (_i, [_vp] * 11 + [_i, _i, _i, _i, _i, _i, _f, _vp]),
     "vv_attn_decode_batch_scratch_bytes": (C.c_size_t, [_i, _i, _i, _i]),
     "vv_attn_decode_batch": (_i, [_i, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _vp, _sz, _vp]),
