@@ -275,7 +275,7 @@ def _own(s):
     if case["op"] == "plan":
         _ok(dev.vv_kv_page_plan_dev(at["new_lens"], at["cache_lens"], s["n"], at["tables"], s["width"], at["free"],
                                     at["n_free"], at["lens"], at["row_starts"], at["positions"], at["slots"], s["rows"],
-                                    at["counts"], stream))
+                                    None, at["counts"], stream))
         return {k: s[k] for k in ("tables", "lens", "row_starts", "positions", "slots", "counts")}
     nq, nkv, hd, fmt = case["q_heads"], case["kv_heads"], case["head_dim"], case["format"]
     if case["op"] == "append":
