@@ -1,6 +1,11 @@
 // Decode attention of many sequences over one paged pool: one query row per sequence and head, each sequence behind its
 // own row of page ids and of its own length, the lengths on the device.
 #include <algorithm>
+#ifndef VVD16
+#define VVD16 2
+#define VVD8 3
+#define VVD64 3
+#endif
 
 #include "attn_common.hpp"
 
@@ -9,9 +14,17 @@ namespace {
 
 constexpr int kBatchThreads = 256;
 constexpr int kBatchWaves = kBatchThreads / kWave;
-constexpr int kWorkers = 1024;
+constexpr int kWorkers = 512;                // workgroups the pages are dealt to: two for each of 256 compute units
 constexpr int kSliceHeads = 16;              // query heads of a group that one workgroup takes: a matrix tile's columns
+constexpr int kSeqChunk = 1024;              // sequences whose lengths a workgroup holds at a time
+// A probability is formed on the scale 2^kLift of the row's maximum, so that it leaves FP16's normal range only 2^24
+// below that; the factor is in the sum of the row too and cancels.
+constexpr float kLift = 10.0f;
+constexpr int kItems = 256;                  // pages whose work a workgroup holds at a time
 
+struct Row {                                 // a row of the work: (sequence, KV head)
+    int first, last;                         // the workers it is dealt to
+};
 struct BatchArgs {
     const h16* q;
     const void* k;
@@ -19,7 +32,7 @@ struct BatchArgs {
     const int* tables;
     const int* lens;
     h16* out;
-    int* starts;            // [n_seqs + 1] pages before each sequence
+    Row* rows;              // [n_seqs * n_kv_heads]
     float* parts;
     int n_q_heads, n_kv_heads, n_seqs, max_pages, n_pages;
     float scale_log2;
@@ -36,267 +49,456 @@ __device__ __forceinline__ int wave_prefix(int v) {       // inclusive
     }
     return v;
 }
+// Exclusive prefix over the workgroup and the sum of all. `sums` is free again after the caller's next barrier.
+__device__ __forceinline__ int block_prefix(int v, int* sums, int& total) {
+    const int incl = wave_prefix(v);
+    if (lane_id() == 63) sums[wave_in_block()] = incl;
+    __syncthreads();
+    int before = incl - v;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kBatchWaves; ++w) {
+        if (w < wave_in_block()) before += sums[w];
+        total += sums[w];
+    }
+    return before;
+}
 
-// A worker's units: [first, last) of the row-major list (sequence, KV head, page).
-__device__ __forceinline__ int units_each(int units) { return (units + kWorkers - 1) / kWorkers; }
-
-// Where a worker leaves the partial state of a stretch: rows that begin inside the worker and run on, or ran on into it.
-__device__ __forceinline__ size_t part_floats(int group_heads, int hd) { return (size_t)group_heads * (hd + 4); }
-
-template <int kHd, int kFmt>
-struct Blocks {             // a wave's sixteen keys as they were loaded
-    static constexpr int kUnit = kFmt == kFmtFp16 ? 2 : 1;
-    static constexpr int kRow = kHd * kUnit;              // bytes per vector
-    static constexpr int kKLoads = kRow / 64;             // 16-byte loads of K per lane
-    Chunk k[kKLoads];
-    Chunk v[4];             // FP8: the lower eight bytes
+// The units (sequence, KV head, page), in that order, dealt to kWorkers workgroups: contiguous runs, the first
+// units % kWorkers of them one longer.
+struct Deal {
+    int q, r;
+    __device__ __forceinline__ explicit Deal(int units) : q(units / kWorkers), r(units % kWorkers) {}
+    __device__ __forceinline__ int begin(int worker) const { return worker * q + min(worker, r); }
+    __device__ __forceinline__ int worker_of(int unit) const {
+        const int longer = r * (q + 1);
+        return unit < longer ? unit / (q + 1) : r + (unit - longer) / max(q, 1);
+    }
 };
 
+// One page of a worker's run, ready to be fetched.
+struct __attribute__((aligned(16))) Item {
+    int page;        // a page of the pool; 0 where the table names none
+    int meta;        // positions in use (0 .. 64), then the flags
+    int seq, kvh;
+};
+constexpr int kFirst = 1 << 8;        // begins a stretch of one row
+constexpr int kLast = 1 << 9;         // ends it
+constexpr int kBegun = 1 << 10;       // the row begins in this worker
+constexpr int kEnded = 1 << 11;       // and ends in it
+
+constexpr int part_floats(int hd) { return hd + 4; }       // a head's partial state: channels, max, sum, 2 unused
+
+// A wave's sixteen positions of a page, as loaded: every load covers whole vectors, 16 bytes a lane. A vector of 256
+// bytes takes sixteen lanes: load i brings positions 4 j + i, j = lane / 16. One of 128 bytes takes eight: load i
+// brings positions 8 i + lane / 8. (Loads in the matrix operand's own layout, sixteen vectors by 64 bytes, stream the
+// cache at 5.0 TB/s - 5.6 without the non-temporal hint - where these reach 6.4.)
 template <int kHd, int kFmt>
-__global__ __launch_bounds__(kBatchThreads, 4) void decode_batch(BatchArgs a) {
-    typedef Blocks<kHd, kFmt> B;
+struct Block {
+    static constexpr int kUnit = kFmt == kFmtFp16 ? 2 : 1;
+    static constexpr int kRow = kHd * kUnit;              // bytes per vector: 128 or 256
+    static constexpr int kLoads = kRow / 64;
+    static constexpr int kRowChunks = kRow / 16;
+    Chunk k[kLoads], v[kLoads];
+};
+
+// A bounded view of memory for buffer loads: a lane whose offset reaches `bytes` or beyond gets zeros and touches nothing.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bounded(const void* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+}
+constexpr int kNonTemporal = 2;          // the cache is read once
+__device__ __forceinline__ Chunk load16(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+    return __builtin_bit_cast(Chunk, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, kNonTemporal));
+}
+
+template <int kHd, int kFmt, int kDepth>
+__global__ __launch_bounds__(kBatchThreads, 2) void decode_batch(BatchArgs a) {
+    typedef Block<kHd, kFmt> B;
     constexpr int kSteps = kHd / 32;                       // 32-channel steps of the score product
-    constexpr int kChunks = kHd / 8;
+    constexpr bool kNarrow = B::kRow == 128;
     constexpr int kTiles = kHd / 16;                       // O^T tiles
-    constexpr int kStride = kHd + 1;
-    __shared__ float o_lds[kBatchWaves][kSliceHeads * kStride];
+    constexpr int kStride = kHd + 4;
+    __shared__ __attribute__((aligned(16))) float o_lds[kBatchWaves][kSliceHeads * kStride];
     __shared__ float m_lds[kBatchWaves][16], l_lds[kBatchWaves][16];
-    __shared__ int s_sum[kBatchWaves], s_at[3];
+    __shared__ Chunk k_lds[kBatchWaves][16 * B::kRowChunks];
+    __shared__ int s_before[kSeqChunk + 1], s_len[kSeqChunk], s_sum[kBatchWaves], s_sum2[kBatchWaves];
+    __shared__ Item s_item[kItems + 2 * kDepth];
 
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = wave_in_block();
     const int c = lane & 15, j = lane >> 4;
     const int worker = (int)blockIdx.x, slice = (int)blockIdx.y;
     const int group = a.n_q_heads / a.n_kv_heads;
     const int heads = min(kSliceHeads, group - slice * kSliceHeads);      // of this slice
+    const uint32_t row_bytes = (uint32_t)a.n_kv_heads * B::kRow;
 
-    // Pages before every sequence.
-    const int each = (a.n_seqs + kBatchThreads - 1) / kBatchThreads;
-    int mine = 0;
-    for (int i = 0; i < each; ++i) {
-        const int s = tid * each + i;
-        if (s < a.n_seqs) mine += pages_of(seen_len(a, s));
+    // More sequences than are held at a time: their pages are summed beforehand.
+    int total = 0;
+    if (a.n_seqs > kSeqChunk) {
+        int mine = 0;
+        for (int s = tid; s < a.n_seqs; s += kBatchThreads) mine += pages_of(seen_len(a, s));
+        block_prefix(mine, s_sum2, total);
     }
-    const int incl = wave_prefix(mine);
-    if (lane == 63) s_sum[wave] = incl;
-    if (tid == 0) { s_at[0] = a.n_seqs; s_at[1] = 0; }
-    __syncthreads();
-    int before = incl - mine, total = 0;
-#pragma unroll
-    for (int w = 0; w < kBatchWaves; ++w) {
-        if (w < wave) before += s_sum[w];
-        total += s_sum[w];
-    }
-    const int units = total * a.n_kv_heads, per = units_each(units);
-    int u = min(worker * per, units);
-    const int u_end = min(u + per, units);
-    if (worker == 0 && slice == 0) {
-        int at = before;
-        for (int i = 0; i < each; ++i) {
-            const int s = tid * each + i;
-            if (s < a.n_seqs) {
-                a.starts[s] = at;
-                at += pages_of(seen_len(a, s));
-            }
-        }
-        if (tid == 0) a.starts[a.n_seqs] = total;
-    }
-    // Sequences without positions: zeros.
-    for (int s = worker; s < a.n_seqs; s += kWorkers) {
-        if (seen_len(a, s) > 0) continue;
-        for (int i = tid; i < heads * a.n_kv_heads * kHd; i += kBatchThreads) {
-            const int kvh = i / (heads * kHd), e = i - kvh * heads * kHd;
-            a.out[((size_t)s * a.n_q_heads + kvh * group + slice * kSliceHeads) * kHd + e] = (h16)0.0f;
-        }
-    }
-    if (u >= u_end) return;
-    // The sequence the first unit lies in.
-    {
-        int at = before;
-        for (int i = 0; i < each; ++i) {
-            const int s = tid * each + i;
-            const int n = s < a.n_seqs ? pages_of(seen_len(a, s)) : 0;
-            if (n > 0 && at * a.n_kv_heads <= u && u < (at + n) * a.n_kv_heads) {
-                s_at[0] = s;
-                s_at[1] = at;
-            }
-            at += n;
-        }
-    }
-    __syncthreads();
-    int seq = s_at[0], unit0 = s_at[1] * a.n_kv_heads;     // its first unit
 
-    while (u < u_end && seq < a.n_seqs) {
-        const int len = seen_len(a, seq), n_pages = pages_of(len);
-        if (n_pages == 0) { ++seq; continue; }
-        const int kvh = (u - unit0) / n_pages, page0 = (u - unit0) - kvh * n_pages;
-        const int page1 = min(n_pages, page0 + (u_end - u));
-        const int* table = a.tables + (size_t)seq * a.max_pages;
-        const size_t row_bytes = (size_t)a.n_kv_heads * B::kRow;
-
-        const int head0 = kvh * group + slice * kSliceHeads;
-        h16x8 qf[kSteps];
-        {
-            const Chunk* qp = reinterpret_cast<const Chunk*>(a.q + ((size_t)seq * a.n_q_heads + head0 + min(c, heads - 1)) * kHd);
+    // The lane's place inside a page, from the vector of the first row and this KV head, for load 0; load i is kLoadRows
+    // rows further.
+    constexpr int kLoadRows = kNarrow ? 8 : 1;
+    const int chunk = lane % B::kRowChunks, row_at = kNarrow ? lane / 8 : 4 * j;
+    uint32_t off[B::kLoads];
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s)
-                qf[s] = __builtin_bit_cast(h16x8, load_chunk(qp + (kFmt == kFmtFp16 ? 4 * s + j : 4 * j + s)));
+    for (int i = 0; i < B::kLoads; ++i) off[i] = (uint32_t)(16 * wave + row_at + i * kLoadRows) * row_bytes + 16u * chunk;
+    // K goes through the wave's own LDS into the matrix operand's layout. Chunk x of position n sits in slot
+    // x ^ n of its row (128-byte rows: x ^ n / 2), so that sixteen lanes write, and read, sixteen different slots.
+    auto k_slot = [&](int n, int x) {
+        return n * B::kRowChunks + (kNarrow ? x ^ ((n >> 1) & 7) : x ^ n);
+    };
+    // The position behind index n of the products: where two loads bring a lane's four positions they are 2 j, 2 j + 1,
+    // 8 + 2 j and 9 + 2 j.
+    auto position = [&](int n) { return kNarrow ? 8 * ((n >> 1) & 1) + 2 * (n >> 2) + (n & 1) : n; };
+
+    B buf[kDepth];
+    h16x8 qn[kDepth][kSteps], qf[kSteps];
+    f32x4 o[kTiles];
+    float m = -INFINITY, l = 0.0f;
+
+    int chunk_units0 = 0;                                  // units before this chunk of sequences
+    for (int c0 = 0; c0 < a.n_seqs; c0 += kSeqChunk) {
+        constexpr int kPer = kSeqChunk / kBatchThreads;
+        int len[kPer], mine = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int s = c0 + tid * kPer + i;
+            len[i] = s < a.n_seqs ? seen_len(a, s) : 0;
         }
-        f32x4 o[kTiles];
 #pragma unroll
-        for (int e = 0; e < kTiles; ++e) o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        float m = -INFINITY, l = 0.0f;
-
-        for (int p = page0; p < page1; ++p) {
-            const int key0 = p * kPage + 16 * wave;        // this wave's sixteen keys
-            const int page = __builtin_amdgcn_readfirstlane(table[p]);
-            const bool bad = page < 0 || page >= a.n_pages;
-            if (key0 >= len || bad) continue;
-            const char* kp = static_cast<const char*>(a.k) + ((size_t)page * kPage + 16 * wave) * row_bytes + (size_t)kvh * B::kRow;
-            const char* vp = static_cast<const char*>(a.v) + ((size_t)page * kPage + 16 * wave) * row_bytes + (size_t)kvh * B::kRow;
-            B b;
+        for (int i = 0; i < kPer; ++i) mine += pages_of(len[i]);
+        int chunk_pages;
+        int before = block_prefix(mine, s_sum, chunk_pages);
 #pragma unroll
-            for (int i = 0; i < B::kKLoads; ++i) {
-                const int at = kFmt == kFmtFp16 ? 64 * i + 16 * j : 32 * j + 16 * i;
-                b.k[i] = load_chunk_stream(reinterpret_cast<const Chunk*>(kp + c * row_bytes + at));
-            }
-            h16x8 v4[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const char* at = vp + (4 * j + i) * row_bytes + (c % kChunks) * (8 * B::kUnit);
-                if constexpr (kFmt == kFmtFp16) {
-                    v4[i] = __builtin_bit_cast(h16x8, load_chunk_stream(reinterpret_cast<const Chunk*>(at)));
-                } else {
-                    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-                    const u32x2 codes = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(at));
-                    Chunk w;
-                    widen4<kFmt>(codes.x, w.w[0], w.w[1]);
-                    widen4<kFmt>(codes.y, w.w[2], w.w[3]);
-                    v4[i] = __builtin_bit_cast(h16x8, w);
-                }
-            }
-            f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                Chunk w;
-                if constexpr (kFmt == kFmtFp16) {
-                    w = b.k[s];
-                } else {
-                    widen4<kFmt>(b.k[s / 2].w[2 * (s & 1)], w.w[0], w.w[1]);
-                    widen4<kFmt>(b.k[s / 2].w[2 * (s & 1) + 1], w.w[2], w.w[3]);
-                }
-                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, w), qf[s], sc, 0, 0, 0);
-            }
-            if (key0 + 16 > len) {                         // what lies past the end is masked, whatever it holds
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool in = key0 + 4 * j + r < len;
-                    sc[r] = in ? sc[r] : -INFINITY;
-                    if (!in) v4[r] = h16x8{0, 0, 0, 0, 0, 0, 0, 0};
-                }
-            }
-            float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-            mx = max_xor32(max_xor16(mx)) * a.scale_log2;
-            const float m_new = fmaxf(m, mx);
-            const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-            const float alpha = exp2_fast(m - m_use);
-            l *= alpha;
-#pragma unroll
-            for (int e = 0; e < kTiles; ++e)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[e][r] *= alpha;
-            m = m_new;
-            h16x4 pf;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float pr = exp2_fast(fmaf(sc[r], a.scale_log2, -m_use));
-                l += pr;
-                pf[r] = (h16)pr;
-            }
-#pragma unroll
-            for (int e = 0; e < kTiles; ++e) {
-                // 128 channels: tile e is the channels 8 c + e. 64: chunk c % 8's channel e + 4 (c / 8).
-                h16x4 vf;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if constexpr (kChunks == 16) vf[r] = v4[r][e];
-                    else vf[r] = c < 8 ? v4[r][e] : v4[r][e + 4];
-                }
-                o[e] = __builtin_amdgcn_mfma_f32_16x16x16f16(vf, pf, o[e], 0, 0, 0);
-            }
+        for (int i = 0; i < kPer; ++i) {
+            s_before[tid * kPer + i] = before;
+            s_len[tid * kPer + i] = len[i];
+            before += pages_of(len[i]);
         }
-
-        // The waves' states meet in LDS.
-        l = sum_xor32(sum_xor16(l));
+        if (tid == 0) s_before[kSeqChunk] = chunk_pages;
+        if (a.n_seqs <= kSeqChunk) total = chunk_pages;
+        const Deal deal(total * a.n_kv_heads);
+        const int u0 = deal.begin(worker), u1 = deal.begin(worker + 1);
         __syncthreads();
-        if (j == 0) { m_lds[wave][c] = m; l_lds[wave][c] = l; }
-        if (c < heads) {
-#pragma unroll
-            for (int e = 0; e < kTiles; ++e)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int tile_row = 4 * j + r;
-                    const int ch = kChunks == 16 ? 8 * tile_row + e : 8 * (tile_row & 7) + e + 4 * (tile_row >> 3);
-                    o_lds[wave][c * kStride + ch] = o[e][r];
+
+        // Sequences without positions: zeros, and a row that nobody shares.
+        for (int s = worker; s < kSeqChunk && c0 + s < a.n_seqs; s += kWorkers) {
+            if (s_len[s] > 0) continue;
+            for (int i = tid; i < heads * a.n_kv_heads * kHd; i += kBatchThreads) {
+                const int kvh = i / (heads * kHd), e = i - kvh * heads * kHd;
+                a.out[((size_t)(c0 + s) * a.n_q_heads + kvh * group + slice * kSliceHeads) * kHd + e] = (h16)0.0f;
+            }
+            if (slice == 0)
+                for (int i = tid; i < a.n_kv_heads; i += kBatchThreads)
+                    a.rows[(size_t)(c0 + s) * a.n_kv_heads + i] = Row{0, 0};
+        }
+
+        const int chunk_units1 = chunk_units0 + chunk_pages * a.n_kv_heads;
+        const int last_unit = min(u1, chunk_units1);
+        for (int base = max(u0, chunk_units0); base < last_unit; base += kItems) {
+            const int n = min(kItems, last_unit - base);
+            if (tid < 2 * kDepth) s_item[n + tid] = Item{0, 0, 0, 0};      // nothing to fetch, nothing to do
+            if (tid < n) {
+                const int u = base + tid, in_chunk = u - chunk_units0;
+                int lo = 0, hi = kSeqChunk - 1;            // the first sequence that ends past the unit
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if (s_before[mid + 1] * a.n_kv_heads > in_chunk) hi = mid;
+                    else lo = mid + 1;
                 }
+                const int n_row = s_before[lo + 1] - s_before[lo];
+                const int rel = in_chunk - s_before[lo] * a.n_kv_heads;
+                const int kvh = rel / n_row, p = rel - kvh * n_row;
+                const int row0 = u - p;                    // the row's first unit
+                int page = a.tables[(size_t)(c0 + lo) * a.max_pages + p];
+                int meta = min(kPage, s_len[lo] - p * kPage);
+                if (page < 0 || page >= a.n_pages) page = meta = 0;
+                if (p == 0 || u == u0) meta |= kFirst;
+                if (p == n_row - 1 || u == u1 - 1) meta |= kLast;
+                if (row0 >= u0) meta |= kBegun;
+                if (row0 + n_row <= u1) meta |= kEnded;
+                s_item[tid] = Item{page, meta, c0 + lo, kvh};
+                if (p == 0 && slice == 0)
+                    a.rows[(size_t)(c0 + lo) * a.n_kv_heads + kvh] = Row{worker, deal.worker_of(row0 + n_row - 1)};
+            }
+            __syncthreads();
+
+            auto item_at = [&](int i) {
+                const Item it = s_item[i];
+                Item u;
+                u.page = __builtin_amdgcn_readfirstlane(it.page);
+                u.meta = __builtin_amdgcn_readfirstlane(it.meta);
+                u.seq = __builtin_amdgcn_readfirstlane(it.seq);
+                u.kvh = __builtin_amdgcn_readfirstlane(it.kvh);
+                return u;
+            };
+            // The positions in use bound the view: what lies past them reads as zeros, and an item of none reads nothing,
+            // so every item, an empty one behind the last too, issues the same loads and the waits can be counted.
+            auto fetch = [&](B& b, h16x8 (&q)[kSteps], int i) {
+                const Item it = item_at(i);
+                const size_t at = (size_t)it.page * kPage * row_bytes + (size_t)it.kvh * B::kRow;
+                const int bytes = max((it.meta & 0xFF) * (int)row_bytes - it.kvh * B::kRow, 0);
+                const auto kp = bounded(static_cast<const char*>(a.k) + at, bytes);
+                const auto vp = bounded(static_cast<const char*>(a.v) + at, bytes);
+#pragma unroll
+                for (int x = 0; x < B::kLoads; ++x) b.k[x] = load16(kp, off[x]);
+#pragma unroll
+                for (int x = 0; x < B::kLoads; ++x) b.v[x] = load16(vp, off[x]);
+                if (it.meta & kFirst) {
+                    const int head = it.kvh * group + slice * kSliceHeads + min(c, heads - 1);
+                    const Chunk* qp = reinterpret_cast<const Chunk*>(a.q + ((size_t)it.seq * a.n_q_heads + head) * kHd);
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s)
+                        q[s] = __builtin_bit_cast(h16x8, load_chunk(qp + (kFmt == kFmtFp16 ? 4 * s + j : 4 * j + s)));
+                }
+            };
+            auto step = [&](const B& b, const h16x8 (&q)[kSteps], int i) {
+                const Item it = item_at(i);
+                const int in_use = (it.meta & 0xFF) - 16 * wave;       // of this wave's sixteen
+                if (it.meta & kFirst) {
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s) qf[s] = q[s];
+#pragma unroll
+                    for (int e = 0; e < kTiles; ++e) o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    m = -INFINITY;
+                    l = 0.0f;
+                }
+                if (in_use > 0) {
+#pragma unroll
+                    for (int x = 0; x < B::kLoads; ++x) k_lds[wave][k_slot(row_at + x * kLoadRows, chunk)] = b.k[x];
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if constexpr (kFmt == kFmtFp16) {
+#pragma unroll
+                        for (int s = 0; s < kSteps; ++s)
+                            sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                __builtin_bit_cast(h16x8, k_lds[wave][k_slot(position(c), 4 * s + j)]), qf[s], sc, 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int s = 0; s < kSteps; s += 2) {
+                            const Chunk codes = k_lds[wave][k_slot(position(c), 2 * j + s / 2)];
+#pragma unroll
+                            for (int z = 0; z < 2; ++z) {
+                                Chunk w;
+                                widen4<kFmt>(codes.w[2 * z], w.w[0], w.w[1]);
+                                widen4<kFmt>(codes.w[2 * z + 1], w.w[2], w.w[3]);
+                                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, w), qf[s + z], sc, 0, 0, 0);
+                            }
+                        }
+                    }
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    // v4[r]: position(4 j + r), the eight channels (four, 64 channels) of this lane's row of the tiles.
+                    h16x8 v4[4];
+                    if constexpr (!kNarrow) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v4[r] = __builtin_bit_cast(h16x8, b.v[r]);
+                    } else {
+                        // Lanes c and c ^ 8 hold the same chunk of positions 2 j and 2 j + 1 (and 8 more): each keeps one
+                        // half of the chunk, the lower lane the lower, and gives away the other.
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            uint32_t keep[2], got[2];
+#pragma unroll
+                            for (int z = 0; z < 2; ++z) {
+                                keep[z] = c < 8 ? b.v[x].w[z] : b.v[x].w[2 + z];
+                                got[z] = (uint32_t)__builtin_amdgcn_update_dpp(
+                                    0, (int)(c < 8 ? b.v[x].w[2 + z] : b.v[x].w[z]), 0x128, 0xF, 0xF, true);   // row_ror:8
+                            }
+#pragma unroll
+                            for (int odd = 0; odd < 2; ++odd) {
+                                const bool own = odd == 0 ? c < 8 : c >= 8;
+                                const uint32_t w0 = own ? keep[0] : got[0], w1 = own ? keep[1] : got[1];
+                                Chunk w = {};
+                                if constexpr (kFmt == kFmtFp16) {
+                                    w.w[0] = w0;
+                                    w.w[1] = w1;
+                                } else {
+                                    widen4<kFmt>(w0, w.w[0], w.w[1]);
+                                    widen4<kFmt>(w1, w.w[2], w.w[3]);
+                                }
+                                v4[2 * x + odd] = __builtin_bit_cast(h16x8, w);
+                            }
+                        }
+                    }
+                    if (in_use < 16) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) sc[r] = position(4 * j + r) < in_use ? sc[r] : -INFINITY;
+                    }
+                    float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+                    mx = max_xor32(max_xor16(mx)) * a.scale_log2;
+                    const float m_new = fmaxf(m, mx);
+                    const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+                    if (__builtin_amdgcn_ballot_w64(m_new > m) != 0) {
+                        const float alpha = exp2_fast(m - m_use);
+                        l *= alpha;
+#pragma unroll
+                        for (int e = 0; e < kTiles; ++e)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) o[e][r] *= alpha;
+                    }
+                    m = m_new;
+                    h16x4 pf;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float pr = exp2_fast(fmaf(sc[r], a.scale_log2, kLift - m_use));
+                        l += pr;
+                        pf[r] = (h16)pr;
+                    }
+#pragma unroll
+                    for (int e = 0; e < kTiles; ++e) {
+                        // Row n of tile e: channel 8 n + e; of 128-byte rows, channel e of what lane n kept.
+                        h16x4 vf;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) vf[r] = v4[r][e];
+                        o[e] = __builtin_amdgcn_mfma_f32_16x16x16f16(vf, pf, o[e], 0, 0, 0);
+                    }
+                }
+                if (it.meta & kLast) {                     // the waves' states meet in LDS
+                    l = sum_xor32(sum_xor16(l));
+                    __syncthreads();                       // the last stretch's states have been read
+                    if (j == 0) { m_lds[wave][c] = m; l_lds[wave][c] = l; }
+                    if (c < heads) {
+#pragma unroll
+                        for (int e = 0; e < kTiles; ++e)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const int tile_row = 4 * j + r;
+                                const int ch = !kNarrow ? 8 * tile_row + e
+                                                        : 2 * kTiles * (tile_row & 7) + kTiles * (tile_row >> 3) + e;
+                                o_lds[wave][c * kStride + ch] = o[e][r];
+                            }
+                    }
+                    __syncthreads();
+                    const int head0 = it.kvh * group + slice * kSliceHeads;
+                    const bool whole = (it.meta & kBegun) && (it.meta & kEnded);
+                    float* dst = a.parts + (((size_t)worker * 2 + (it.meta & kBegun ? 1 : 0)) * gridDim.y + slice) *
+                                               min(group, kSliceHeads) * part_floats(kHd);
+                    // Four channels a thread, whole heads side by side; no loop, so that the loads in flight stay so.
+                    constexpr int kQuads = kHd / 4, kAtOnce = kBatchThreads / kQuads;
+#pragma unroll
+                    for (int pass = 0; pass < kSliceHeads / kAtOnce; ++pass) {
+                        const int h = tid / kQuads + pass * kAtOnce, ch = 4 * (tid % kQuads);
+                        if (h >= heads) continue;
+                        float m_all = -INFINITY;
+#pragma unroll
+                        for (int w = 0; w < kBatchWaves; ++w) m_all = fmaxf(m_all, m_lds[w][h]);
+                        f32x4 ov = {0.0f, 0.0f, 0.0f, 0.0f};
+                        float l_all = 0.0f;
+#pragma unroll
+                        for (int w = 0; w < kBatchWaves; ++w) {
+                            const float mw = m_lds[w][h];
+                            const float f = mw == -INFINITY ? 0.0f : exp2_fast(mw - m_all);
+                            const f32x4 ow = *reinterpret_cast<const f32x4*>(&o_lds[w][h * kStride + ch]);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) ov[r] = fmaf(ow[r], f, ov[r]);
+                            l_all = fmaf(l_lds[w][h], f, l_all);
+                        }
+                        if (whole) {
+                            h16* to = a.out + ((size_t)it.seq * a.n_q_heads + head0 + h) * kHd + ch;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) to[r] = to_half(l_all == 0.0f ? 0.0f : ov[r] / l_all);
+                        } else {
+                            float* rec = dst + (size_t)h * part_floats(kHd);
+                            *reinterpret_cast<f32x4*>(rec + ch) = ov;
+                            if (ch == 0) { rec[kHd] = m_all; rec[kHd + 1] = l_all; }
+                        }
+                    }
+                }
+            };
+
+#pragma unroll
+            for (int d = 0; d < kDepth; ++d) fetch(buf[d], qn[d], d);
+            for (int i = 0; i < n; i += kDepth) {
+#pragma unroll
+                for (int d = 0; d < kDepth; ++d) {
+                    step(buf[d], qn[d], i + d);
+                    fetch(buf[d], qn[d], i + d + kDepth);
+                }
+            }
+            __syncthreads();                               // the items are free again
         }
+        chunk_units0 = chunk_units1;
         __syncthreads();
-        const bool whole = page0 == 0 && page1 == n_pages;
-        float* dst = a.parts + (((size_t)worker * 2 + (page0 == 0 ? 1 : 0)) * gridDim.y + slice) *
-                                   part_floats(min(group, kSliceHeads), kHd);
-        for (int i = tid; i < heads * kHd; i += kBatchThreads) {
-            const int h = i / kHd, ch = i % kHd;
-            float m_all = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kBatchWaves; ++w) m_all = fmaxf(m_all, m_lds[w][h]);
-            float ov = 0.0f, l_all = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kBatchWaves; ++w) {
-                const float mw = m_lds[w][h];
-                const float f = mw == -INFINITY ? 0.0f : exp2_fast(mw - m_all);
-                ov = fmaf(o_lds[w][h * kStride + ch], f, ov);
-                l_all = fmaf(l_lds[w][h], f, l_all);
-            }
-            if (whole) {
-                a.out[((size_t)seq * a.n_q_heads + head0 + h) * kHd + ch] = to_half(l_all == 0.0f ? 0.0f : ov / l_all);
-            } else {
-                float* rec = dst + (size_t)h * (kHd + 4);
-                rec[ch] = ov;
-                if (ch == 0) { rec[kHd] = m_all; rec[kHd + 1] = l_all; }
-            }
-        }
-        u += page1 - page0;
-        if (u == unit0 + n_pages * a.n_kv_heads) { ++seq; unit0 = u; }
     }
 }
 
-// Folds the stretches of a row (sequence, KV head) that several workers share.
-template <int kHd>
-__global__ __launch_bounds__(256) void decode_batch_merge(BatchArgs a, int slices) {
+// Folds the partial states of the rows that several workers share, in the order of their pages. A thread holds four
+// channels of one head over every kGroups-th part; the groups' states meet in LDS.
+template <int kHd, int kGroups>
+__global__ void decode_batch_merge(BatchArgs a, int slices, int heads_per_wg) {
+    constexpr int kQuads = kHd / 4;
+    __shared__ float s_m[kGroups], s_l[kGroups];
+    __shared__ __attribute__((aligned(16))) float s_o[kGroups > 1 ? kGroups * kHd : 1];
     const int group = a.n_q_heads / a.n_kv_heads;
-    const int seq = (int)blockIdx.x, head = (int)blockIdx.y, kvh = head / group, in_group = head - kvh * group;
+    const int row = (int)blockIdx.x, per = min(group, kSliceHeads);
+    const Row at = a.rows[row];
+    if (at.first == at.last) return;                                     // that worker wrote the output
+    const int quad = (int)threadIdx.x % kQuads;
+    const int rest = (int)threadIdx.x / kQuads;
+    const int grp = kGroups > 1 ? rest : 0;
+    const int in_group = (int)blockIdx.y * heads_per_wg + (kGroups > 1 ? 0 : rest);
+    if (kGroups == 1 && (rest >= heads_per_wg || in_group >= group)) return;
     const int slice = in_group / kSliceHeads, h = in_group - slice * kSliceHeads;
-    const int total = a.starts[a.n_seqs] * a.n_kv_heads, per = units_each(total);
-    const int pages = a.starts[seq + 1] - a.starts[seq];
-    if (pages == 0) return;
-    const int u0 = a.starts[seq] * a.n_kv_heads + kvh * pages, u1 = u0 + pages;
-    const int first = u0 / per, last = (u1 - 1) / per;
-    if (first == last) return;                                     // that worker wrote the output
-    const size_t record = part_floats(min(group, kSliceHeads), kHd);
     auto part = [&](int w) {
-        return a.parts + (((size_t)w * 2 + (w == first ? 1 : 0)) * slices + slice) * record + (size_t)h * (kHd + 4);
+        return a.parts + ((((size_t)w * 2 + (w == at.first ? 1 : 0)) * slices + slice) * per + h) * part_floats(kHd);
     };
-    const int ch = (int)threadIdx.x;
-    if (ch >= kHd) return;
-    float m_all = -INFINITY;
-    for (int w = first; w <= last; ++w) m_all = fmaxf(m_all, part(w)[kHd]);
-    float o = 0.0f, l = 0.0f;
-    for (int w = first; w <= last; ++w) {
-        const float* p = part(w);
-        const float f = p[kHd] == -INFINITY ? 0.0f : exp2_fast(p[kHd] - m_all);
-        o = fmaf(p[ch], f, o);
-        l = fmaf(p[kHd + 1], f, l);
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    constexpr int kAhead = 8;
+    for (int w0 = at.first + grp; w0 <= at.last; w0 += kAhead * kGroups) {
+        f32x4 ov[kAhead];
+        float mv[kAhead], lv[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int w = w0 + i * kGroups;
+            const float* p = part(min(w, at.last));
+            ov[i] = *reinterpret_cast<const f32x4*>(p + 4 * quad);
+            mv[i] = w <= at.last ? p[kHd] : -INFINITY;
+            lv[i] = p[kHd + 1];
+        }
+        float m_new = m;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) m_new = fmaxf(m_new, mv[i]);
+        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+        const float keep = exp2_fast(m - m_use);
+        o *= keep;
+        l *= keep;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (mv[i] == -INFINITY) continue;              // nothing seen there: no part of the sums, whatever it holds
+            const float f = exp2_fast(mv[i] - m_use);
+            l = fmaf(lv[i], f, l);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = fmaf(ov[i][r], f, o[r]);
+        }
+        m = m_new;
     }
-    a.out[((size_t)seq * a.n_q_heads + head) * kHd + ch] = to_half(l == 0.0f ? 0.0f : o / l);
+    if constexpr (kGroups > 1) {
+        if (quad == 0) { s_m[grp] = m; s_l[grp] = l; }
+        *reinterpret_cast<f32x4*>(&s_o[grp * kHd + 4 * quad]) = o;
+        __syncthreads();
+        if (grp > 0) return;
+        for (int g = 0; g < kGroups; ++g) m = fmaxf(m, s_m[g]);
+        const float m_use = m == -INFINITY ? 0.0f : m;
+        o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        l = 0.0f;
+#pragma unroll 8
+        for (int g = 0; g < kGroups; ++g) {
+            const float f = exp2_fast(s_m[g] - m_use);
+            const f32x4 og = *reinterpret_cast<const f32x4*>(&s_o[g * kHd + 4 * quad]);
+            l = fmaf(s_l[g], f, l);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = fmaf(og[r], f, o[r]);
+        }
+    }
+    const int seq = row / a.n_kv_heads, kvh = row - seq * a.n_kv_heads;
+    h16* dst = a.out + ((size_t)seq * a.n_q_heads + kvh * group + in_group) * kHd + 4 * quad;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) dst[r] = to_half(l == 0.0f ? 0.0f : o[r] / l);
 }
 
 // Any head_dim <= 256, any alignment, FP16: a wave per (sequence, head) walks the sequence's keys.
@@ -343,7 +545,28 @@ __global__ __launch_bounds__(kWave) void decode_batch_generic(BatchArgs a, int h
     }
 }
 
-inline size_t starts_bytes(int n_seqs) { return (((size_t)n_seqs + 1) * sizeof(int) + 255) & ~(size_t)255; }
+inline size_t row_bytes(int n_seqs, int n_kv_heads) {
+    return ((size_t)n_seqs * n_kv_heads * sizeof(Row) + 255) & ~(size_t)255;
+}
+
+template <int kHd, int kFmt, int kDepth>
+void launch(const BatchArgs& a, int slices, hipStream_t st) {
+    decode_batch<kHd, kFmt, kDepth><<<dim3(kWorkers, (unsigned)slices), kBatchThreads, 0, st>>>(a);
+}
+
+template <int kHd>
+void launch_merge(const BatchArgs& a, int slices, hipStream_t st) {
+    const int rows = a.n_seqs * a.n_kv_heads, group = a.n_q_heads / a.n_kv_heads;
+    constexpr int kMany = 1024 / (kHd / 4);
+    if (rows <= 32) {
+        decode_batch_merge<kHd, kMany><<<dim3((unsigned)rows, (unsigned)group), 1024, 0, st>>>(a, slices, 1);
+    } else {
+        const int heads = std::min(group, 8);
+        const unsigned threads = (unsigned)(heads * (kHd / 4) + kWave - 1) / kWave * kWave;
+        decode_batch_merge<kHd, 1><<<dim3((unsigned)rows, (unsigned)((group + heads - 1) / heads)), threads, 0, st>>>(
+            a, slices, heads);
+    }
+}
 
 }  // namespace
 }  // namespace vv
@@ -353,8 +576,8 @@ extern "C" {
 size_t vv_attn_decode_batch_scratch_bytes(int n_seqs, int n_q_heads, int n_kv_heads, int head_dim) {
     if (n_seqs <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || n_q_heads % n_kv_heads) return 0;
     const int group = n_q_heads / n_kv_heads, slices = (group + vv::kSliceHeads - 1) / vv::kSliceHeads;
-    return vv::starts_bytes(n_seqs) + (size_t)vv::kWorkers * 2 * slices * std::min(group, vv::kSliceHeads) *
-                                          ((size_t)head_dim + 4) * sizeof(float);
+    return vv::row_bytes(n_seqs, n_kv_heads) + (size_t)vv::kWorkers * 2 * slices * std::min(group, vv::kSliceHeads) *
+                                                   vv::part_floats(head_dim) * sizeof(float);
 }
 
 vv_status_t vv_attn_decode_batch(int backend, const void* q, const vv_kv_view_t* kv, void* out, int n_q_heads,
@@ -366,7 +589,7 @@ vv_status_t vv_attn_decode_batch(int backend, const void* q, const vv_kv_view_t*
     if (!kv->k || !kv->v || !kv->page_table) return VV_ERR_NULL_PTR;
     const bool fp8 = kv->format == vv::kFmtE4M3 || kv->format == vv::kFmtE5M2;
     if (kv->format != vv::kFmtFp16 && !(fp8 && kv->head_dim == 128)) return VV_ERR_UNSUPPORTED;
-    if (n_q_heads <= 0 || kv->n_kv_heads <= 0 || n_q_heads % kv->n_kv_heads || kv->head_dim <= 0 || kv->head_dim > 256)
+    if (n_q_heads <= 0 || n_q_heads > 65535 || kv->n_kv_heads <= 0 || n_q_heads % kv->n_kv_heads || kv->head_dim <= 0 || kv->head_dim > 256)
         return VV_ERR_UNSUPPORTED;
     if (max_pages <= 0 || n_pages <= 0) return VV_ERR_INVALID_ARG;
     // the list of (sequence, KV head, page) is counted in 32 bits
@@ -382,23 +605,16 @@ vv_status_t vv_attn_decode_batch(int backend, const void* q, const vv_kv_view_t*
         const size_t want = vv_attn_decode_batch_scratch_bytes(n_seqs, n_q_heads, kv->n_kv_heads, kv->head_dim);
         if (!scratch) return VV_ERR_NULL_PTR;
         if (scratch_bytes < want || !vv::aligned16(scratch)) return VV_ERR_INVALID_ARG;
-        a.starts = static_cast<int*>(scratch);
-        a.parts = reinterpret_cast<float*>(static_cast<char*>(scratch) + vv::starts_bytes(n_seqs));
+        a.rows = static_cast<vv::Row*>(scratch);
+        a.parts = reinterpret_cast<float*>(static_cast<char*>(scratch) + vv::row_bytes(n_seqs, kv->n_kv_heads));
         const int group = n_q_heads / kv->n_kv_heads, slices = (group + vv::kSliceHeads - 1) / vv::kSliceHeads;
-        const dim3 grid(vv::kWorkers, (unsigned)slices), merge((unsigned)n_seqs, (unsigned)n_q_heads);
-        if (kv->head_dim == 64)
-            vv::decode_batch<64, vv::kFmtFp16><<<grid, vv::kBatchThreads, 0, st>>>(a);
-        else if (kv->format == vv::kFmtFp16)
-            vv::decode_batch<128, vv::kFmtFp16><<<grid, vv::kBatchThreads, 0, st>>>(a);
-        else if (kv->format == vv::kFmtE4M3)
-            vv::decode_batch<128, vv::kFmtE4M3><<<grid, vv::kBatchThreads, 0, st>>>(a);
-        else
-            vv::decode_batch<128, vv::kFmtE5M2><<<grid, vv::kBatchThreads, 0, st>>>(a);
+        if (kv->head_dim == 64) vv::launch<64, vv::kFmtFp16, VVD64>(a, slices, st);
+        else if (kv->format == vv::kFmtFp16) vv::launch<128, vv::kFmtFp16, VVD16>(a, slices, st);
+        else if (kv->format == vv::kFmtE4M3) vv::launch<128, vv::kFmtE4M3, VVD8>(a, slices, st);
+        else vv::launch<128, vv::kFmtE5M2, VVD8>(a, slices, st);
         if (hipGetLastError() != hipSuccess) return VV_ERR_CUDA_LAUNCH;
-        if (kv->head_dim == 64)
-            vv::decode_batch_merge<64><<<merge, 64, 0, st>>>(a, slices);
-        else
-            vv::decode_batch_merge<128><<<merge, 128, 0, st>>>(a, slices);
+        if (kv->head_dim == 64) vv::launch_merge<64>(a, slices, st);
+        else vv::launch_merge<128>(a, slices, st);
     } else {
         const dim3 grid((unsigned)n_seqs, (unsigned)n_q_heads);
         vv::decode_batch_generic<<<grid, vv::kWave, 0, st>>>(a, kv->head_dim);
