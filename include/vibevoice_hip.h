@@ -679,7 +679,7 @@ vv_status_t vv_kv_page_plan_dev(const int* new_lens, const int* cache_lens, int 
  * [n_rows][n_kv_heads][head_dim] FP16; a bias may be NULL. FP32 arithmetic and one rounding to FP16, of which an FP8
  * pool takes the code: without biases the bits are those of vv_rope_qk_dev and vv_kv_store_dev (without a reference
  * key) on each row; with them q and K are spared the rounding that vv_bias_add_dev does before the rotation.
- * A row whose slot is negative or not below 64 * n_pages is skipped: nothing of it is read or written, q_out
+ * A row whose slot is negative or not below 64 * n_pages is skipped: nothing of it is written, its row of q_out
  * included. Slots must differ from one another; of two rows with one slot either may win, vector piece by piece.
  * kv_format FP16: any even head_dim <= 256 and 2-byte alignment (head_dim 64 and 128 with everything 16-byte aligned
  * take the vector kernel); FP8 E4M3 / E5M2: head_dim 128, 16-byte aligned tensors, 8-byte aligned stores. Other

@@ -14,7 +14,11 @@ namespace {
 
 constexpr int kBatchThreads = 256;
 constexpr int kBatchWaves = kBatchThreads / kWave;
-constexpr int kWorkers = 512;                // workgroups the pages are dealt to: two for each of 256 compute units
+#ifndef VVW
+#define VVW 512
+#define VVOCC 2
+#endif
+constexpr int kWorkers = VVW;                // workgroups the pages are dealt to: two for each of 256 compute units
 constexpr int kSliceHeads = 16;              // query heads of a group that one workgroup takes: a matrix tile's columns
 constexpr int kSeqChunk = 1024;              // sequences whose lengths a workgroup holds at a time
 // A probability is formed on the scale 2^kLift of the row's maximum, so that it leaves FP16's normal range only 2^24
@@ -41,13 +45,17 @@ struct BatchArgs {
 __device__ __forceinline__ int seen_len(const BatchArgs& a, int s) { return min(max(a.lens[s], 0), a.max_pages * kPage); }
 __device__ __forceinline__ int pages_of(int len) { return (len + kPage - 1) / kPage; }
 
-__device__ __forceinline__ int wave_prefix(int v) {       // inclusive
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const int o = __shfl_up(v, d);
-        if (lane_id() >= d) v += o;
-    }
-    return v;
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int add_lane(int v) { return v + __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xF, false); }
+// Inclusive prefix over the wave, in the vector ALU: shifts by 1, 2, 4, 8 within rows of sixteen lanes, then the last
+// lane of a row into the next row, then of the first half into the second.
+__device__ __forceinline__ int wave_prefix(int v) {
+    v = add_lane<0x111, 0xF>(v);
+    v = add_lane<0x112, 0xF>(v);
+    v = add_lane<0x114, 0xF>(v);
+    v = add_lane<0x118, 0xF>(v);
+    v = add_lane<0x142, 0xA>(v);
+    return add_lane<0x143, 0xC>(v);
 }
 // Exclusive prefix over the workgroup and the sum of all. `sums` is free again after the caller's next barrier.
 __device__ __forceinline__ int block_prefix(int v, int* sums, int& total) {
@@ -112,7 +120,7 @@ __device__ __forceinline__ Chunk load16(__amdgpu_buffer_rsrc_t r, uint32_t at) {
 }
 
 template <int kHd, int kFmt, int kDepth>
-__global__ __launch_bounds__(kBatchThreads, 2) void decode_batch(BatchArgs a) {
+__global__ __launch_bounds__(kBatchThreads, VVOCC) void decode_batch(BatchArgs a) {
     typedef Block<kHd, kFmt> B;
     constexpr int kSteps = kHd / 32;                       // 32-channel steps of the score product
     constexpr bool kNarrow = B::kRow == 128;
@@ -204,7 +212,7 @@ __global__ __launch_bounds__(kBatchThreads, 2) void decode_batch(BatchArgs a) {
             if (tid < 2 * kDepth) s_item[n + tid] = Item{0, 0, 0, 0};      // nothing to fetch, nothing to do
             if (tid < n) {
                 const int u = base + tid, in_chunk = u - chunk_units0;
-                int lo = 0, hi = kSeqChunk - 1;            // the first sequence that ends past the unit
+                int lo = 0, hi = min(kSeqChunk, a.n_seqs - c0) - 1;      // the first sequence that ends past the unit
                 while (lo < hi) {
                     const int mid = (lo + hi) >> 1;
                     if (s_before[mid + 1] * a.n_kv_heads > in_chunk) hi = mid;

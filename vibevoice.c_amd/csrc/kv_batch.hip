@@ -163,9 +163,10 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan(PlanArgs a) {
 // off by sqrt(2) as much). The angle and the rotation are those of vv_rope_dev, and an FP8 code is that of the
 // FP16 value, so without biases the bits are those of vv_rope_qk_dev and vv_kv_store_dev on that row. A row moves 4 hd (nq + nkv) + 2 hd nkv (1 + bytes per stored value) bytes and does
 // three flops a value: bound by memory, or by its latency when there are few rows.
-// A lane's item is one pair of chunks (c, c + hd/16) of one head: the eight rotary pairs (d, d + hd/2), or for V just
-// sixteen values. Heads are counted q, then k, then v. A row takes `waves` waves; each computes the row's hd/2
-// cosines and sines, one pair per lane, and collects the eight a lane needs by lane exchange - no LDS, no barrier.
+// A thread's item is one pair of chunks (c, c + hd/16) of one head: the eight rotary pairs (d, d + hd/2), or for V just
+// sixteen values. Heads are counted q, then k, then v. A workgroup owns whole rows, one where a row has 128 items or
+// more: its threads ask for their items first, then compute the rows' cosines and sines, one pair a thread, into LDS
+// under the loads, and rotate and store behind one barrier.
 struct AppendArgs {
     const h16* q;
     const h16* k;
@@ -182,75 +183,89 @@ struct AppendArgs {
     int rows, nq, nkv, head_dim;
 };
 
-template <int kFmt>
+template <int kFmt, bool kStream>
 __device__ __forceinline__ void store_values(void* store, size_t at, const Chunk& c) {      // eight, at element `at`
     if constexpr (kFmt == kFmtFp16) {
-        store_chunk(reinterpret_cast<Chunk*>(static_cast<h16*>(store) + at), c);
+        store_chunk_as<kStream>(reinterpret_cast<Chunk*>(static_cast<h16*>(store) + at), c);
     } else {
         typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
         const h16x8 h = __builtin_bit_cast(h16x8, c);
         u32x2 w = {0u, 0u};
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i >> 2] |= fp8_encode<kFmt == kFmtE5M2>((float)h[i]) << (8 * (i & 3));
-        *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(store) + at) = w;
+        u32x2* dst = reinterpret_cast<u32x2*>(static_cast<uint8_t*>(store) + at);
+        if constexpr (kStream) __builtin_nontemporal_store(w, dst);
+        else *dst = w;
     }
 }
 
-template <int kHd, int kFmt>
-__global__ __launch_bounds__(kBlock) void append_rows(AppendArgs a, FreqTable freqs, int waves) {
-    constexpr int kItems = kHd / 16;              // items per head
-    constexpr int kHeads = kWave / kItems;        // heads a wave takes at a time
-    const int unit = (int)blockIdx.x * kWavesPerBlock + wave_in_block();
-    const int row = unit / waves, part = unit - row * waves;
-    if (row >= a.rows) return;                    // whole waves leave; nothing below synchronises
-    const int64_t slot = a.slots[row];
-    if (slot < 0 || slot >= a.n_slots) return;
-    const int lane = lane_id(), c = lane % kItems;
-    const int heads = a.nq + 2 * a.nkv;
+constexpr int kAppendThreads = 1024;      // at most
+constexpr int kAppendRows = 8;            // rows a workgroup owns, at most
 
-    float my_s, my_c;
-    sincosf((float)a.positions[row] * freqs.f[lane % (kHd / 2)], &my_s, &my_c);
-    f32x8 cv, sv;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        cv[i] = __shfl(my_c, 8 * c + i);
-        sv[i] = __shfl(my_s, 8 * c + i);
-    }
-    for (int head = part * kHeads + lane / kItems; head < heads; head += waves * kHeads) {
+template <int kHd, int kFmt, bool kStream>
+__global__ __launch_bounds__(kAppendThreads) void append_rows(AppendArgs a, FreqTable freqs, int rows_per_wg) {
+    constexpr int kItems = kHd / 16, kHalf = kHd / 2;
+    __shared__ __attribute__((aligned(16))) float cs_cos[kAppendRows * kHalf], cs_sin[kAppendRows * kHalf];
+    const int tid = (int)threadIdx.x;
+    const int row0 = (int)blockIdx.x * rows_per_wg, rows = min(rows_per_wg, a.rows - row0);
+    const int per_row = (a.nq + 2 * a.nkv) * kItems, items = rows * per_row;
+    for (int base = 0; base < items; base += (int)blockDim.x) {       // one round unless a row has more than 1024 items
+        const int item = min(base + tid, items - 1);
+        const int r = rows_per_wg == 1 ? 0 : item / per_row, in_row = item - r * per_row;
+        const int head = in_row / kItems, c = in_row % kItems;
         const int kind = head < a.nq ? 0 : head < a.nq + a.nkv ? 1 : 2;
         const int h = kind == 0 ? head : kind == 1 ? head - a.nq : head - a.nq - a.nkv;
-        const h16* src = kind == 0 ? a.q + (size_t)row * a.nq * kHd
-                                   : (kind == 1 ? a.k : a.v) + (size_t)row * a.nkv * kHd;
+        const size_t row = (size_t)(row0 + r);
+        const h16* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + (row * (kind == 0 ? a.nq : a.nkv) + h) * kHd;
         const h16* bias = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
-        const Chunk* p = reinterpret_cast<const Chunk*>(src + h * kHd) + c;
-        f32x8 x0 = unpack(load_chunk(p)), x1 = unpack(load_chunk(p + kItems));
+        const Chunk* p = reinterpret_cast<const Chunk*>(src) + c;
+        const Chunk lo = load_chunk_as<kStream>(p), hi = load_chunk_as<kStream>(p + kItems);
+        const int64_t slot = a.slots[row];
+        Chunk b0 = {}, b1 = {};
         if (bias) {
-            const Chunk* bp = reinterpret_cast<const Chunk*>(bias + h * kHd) + c;
-            const f32x8 b0 = unpack(load_chunk(bp)), b1 = unpack(load_chunk(bp + kItems));
+            const Chunk* bp = reinterpret_cast<const Chunk*>(bias + (size_t)h * kHd) + c;
+            b0 = load_chunk(bp);
+            b1 = load_chunk(bp + kItems);
+        }
+        if (base == 0) {
+            for (int i = tid; i < rows * kHalf; i += (int)blockDim.x) {
+                float s, cc;
+                sincosf((float)a.positions[row0 + i / kHalf] * freqs.f[i % kHalf], &s, &cc);
+                cs_cos[i] = cc;
+                cs_sin[i] = s;
+            }
+            __syncthreads();
+        }
+        f32x8 x0 = unpack(lo), x1 = unpack(hi);
+        if (bias) {
+            const f32x8 y0 = unpack(b0), y1 = unpack(b1);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                x0[i] += b0[i];
-                x1[i] += b1[i];
+                x0[i] += y0[i];
+                x1[i] += y1[i];
             }
         }
         if (kind != 2) {
+            const f32x8 cv = *reinterpret_cast<const f32x8*>(&cs_cos[r * kHalf + 8 * c]);
+            const f32x8 sv = *reinterpret_cast<const f32x8*>(&cs_sin[r * kHalf + 8 * c]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const Pair r = rotate(x0[i], x1[i], cv[i], sv[i]);
-                x0[i] = r.lo;
-                x1[i] = r.hi;
+                const Pair y = rotate(x0[i], x1[i], cv[i], sv[i]);
+                x0[i] = y.lo;
+                x1[i] = y.hi;
             }
         }
-        const Chunk lo = pack(x0), hi = pack(x1);
+        if (base + tid >= items || slot < 0 || slot >= a.n_slots) continue;
+        const Chunk y0 = pack(x0), y1 = pack(x1);
         if (kind == 0) {
-            Chunk* dst = reinterpret_cast<Chunk*>(a.q_out + ((size_t)row * a.nq + h) * kHd) + c;
-            store_chunk(dst, lo);
-            store_chunk(dst + kItems, hi);
+            Chunk* dst = reinterpret_cast<Chunk*>(a.q_out + (row * a.nq + h) * kHd) + c;
+            store_chunk_as<kStream>(dst, y0);
+            store_chunk_as<kStream>(dst + kItems, y1);
         } else {
             void* store = kind == 1 ? a.k_store : a.v_store;
             const size_t at = ((size_t)slot * a.nkv + h) * kHd + 8 * c;
-            store_values<kFmt>(store, at, lo);
-            store_values<kFmt>(store, at + kHd / 2, hi);
+            store_values<kFmt, kStream>(store, at, y0);
+            store_values<kFmt, kStream>(store, at + kHalf, y1);
         }
     }
 }
@@ -351,17 +366,24 @@ vv_status_t vv_rope_kv_append_dev(const void* q, const void* k, const void* v, c
                              : vv::aligned16(k_store) && vv::aligned16(v_store));
     if (fp8 && !chunks) return VV_ERR_UNSUPPORTED;
     if (chunks && (head_dim == 128 || head_dim == 64)) {
-        const int waves = 1;
-        const int64_t wgs = ((int64_t)n_rows * waves + vv::kWavesPerBlock - 1) / vv::kWavesPerBlock;
-        const dim3 grid((unsigned)wgs);
-        if (head_dim == 64)
-            vv::append_rows<64, vv::kFmtFp16><<<grid, vv::kBlock, 0, st>>>(a, freqs, waves);
-        else if (!fp8)
-            vv::append_rows<128, vv::kFmtFp16><<<grid, vv::kBlock, 0, st>>>(a, freqs, waves);
-        else if (kv_format == vv::kFmtE4M3)
-            vv::append_rows<128, vv::kFmtE4M3><<<grid, vv::kBlock, 0, st>>>(a, freqs, waves);
-        else
-            vv::append_rows<128, vv::kFmtE5M2><<<grid, vv::kBlock, 0, st>>>(a, freqs, waves);
+        const int64_t per_row = (int64_t)(n_q_heads + 2 * n_kv_heads) * (head_dim / 16);
+        int rows = per_row >= 128 ? 1 : (int)(256 / per_row);
+        if (rows > vv::kAppendRows) rows = vv::kAppendRows;
+        if (rows > n_rows) rows = n_rows;
+        const int64_t want = (rows * per_row + vv::kWave - 1) / vv::kWave * vv::kWave;
+        const unsigned threads = (unsigned)(want < vv::kAppendThreads ? want : vv::kAppendThreads);
+        const dim3 grid((unsigned)((n_rows - 1) / rows + 1));
+        const bool stream = vv::use_streaming(2u * (size_t)n_rows * (size_t)per_row * 32u);
+#define VV_APPEND(H, F)                                                                                \
+    do {                                                                                               \
+        if (stream) vv::append_rows<H, vv::F, true><<<grid, threads, 0, st>>>(a, freqs, rows);         \
+        else        vv::append_rows<H, vv::F, false><<<grid, threads, 0, st>>>(a, freqs, rows);        \
+    } while (0)
+        if (head_dim == 64)                       VV_APPEND(64, kFmtFp16);
+        else if (!fp8)                            VV_APPEND(128, kFmtFp16);
+        else if (kv_format == vv::kFmtE4M3)       VV_APPEND(128, kFmtE4M3);
+        else                                      VV_APPEND(128, kFmtE5M2);
+#undef VV_APPEND
     } else {
         vv::append_generic<<<dim3((unsigned)n_rows), vv::kBlock, 0, st>>>(a, freqs);
     }
