@@ -267,6 +267,24 @@ def test_append_against_the_formula(fmt):
         assert (np.abs(got - want) <= off).all(), name
 
 
+@pytest.mark.parametrize("fmt", [E4M3, E5M2])
+def test_append_codes_of_every_half(fmt):
+    """All 65536 FP16 patterns as values: the codes are those of vv_kv_store_dev."""
+    rows, nkv, hd, n_pages = 128, 4, 128, 2
+    v = torch.arange(65536, dtype=torch.int32, device="cuda").to(torch.int16).view(torch.float16).view(rows, nkv, hd)
+    q, k, out = (torch.zeros(rows, n, hd, dtype=torch.float16, device="cuda") for n in (4, nkv, 4))
+    want, got = new_store(n_pages, nkv, hd, fmt), new_store(n_pages, nkv, hd, fmt)
+    wk, gk = new_store(n_pages, nkv, hd, fmt), new_store(n_pages, nkv, hd, fmt)
+    ok(dev.vv_kv_store_dev(k.data_ptr(), v.data_ptr(), wk.data_ptr(), want.data_ptr(), None, None, None, False, nkv, hd, 0,
+                           None, rows, fmt, None, stream()))
+    pos, slots = ints(np.arange(rows)), ints(np.arange(rows), torch.int64)
+    ok(dev.vv_rope_kv_append_dev(q.data_ptr(), k.data_ptr(), v.data_ptr(), None, None, None, pos.data_ptr(),
+                                 slots.data_ptr(), out.data_ptr(), gk.data_ptr(), got.data_ptr(), rows, 4, nkv, hd, n_pages,
+                                 fmt, 1e6, stream()))
+    # (the keys, zeros, were stored there without a rotation, which may turn the sign of a zero)
+    assert np.array_equal(raw(got), raw(want)) and np.array_equal(raw(gk) & 0x7F, raw(wk))
+
+
 @pytest.mark.parametrize("which", range(7))
 def test_append_unaligned(which):
     """Any one FP16 tensor off 16 bytes: the 2-byte kernel, the same bits."""

@@ -166,7 +166,11 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan(PlanArgs a) {
 // A thread's item is one pair of chunks (c, c + hd/16) of one head: the eight rotary pairs (d, d + hd/2), or for V just
 // sixteen values. Heads are counted q, then k, then v. A workgroup owns whole rows, one where a row has 128 items or
 // more: its threads ask for their items first, then compute the rows' cosines and sines, one pair a thread, into LDS
-// under the loads, and rotate and store behind one barrier.
+// under the loads, and rotate and store behind one barrier. Launches of 2 MiB and more store non-temporally (14449
+// rows: 47.3 us, 55 without) but load ordinarily: q, k and v were just written by the projections, and what of them is
+// still cached is worth more than the hint (4096 rows: 12.7 us, 15.2 with it; 14449 rows 47.3 and 46.7). Measured at
+// 28 + 4 heads of 128 with biases: 16 rows 4.0 us, 2161 rows into an E4M3 pool 8.9, 4096 rows 12.7 (6.0 TB/s), 14449 rows
+// 47.3 us (5.6 TB/s; 44.3 without biases).
 struct AppendArgs {
     const h16* q;
     const h16* k;
@@ -183,6 +187,25 @@ struct AppendArgs {
     int rows, nq, nkv, head_dim;
 };
 
+// fp8_encode of a value that is an FP16 value already, without branches, on its bits. E5M2 is the top byte of FP16 and
+// E4M3 its exponent less 8 with three bits of mantissa, so from the smallest normal on a code is those bits rounded to
+// nearest even (a carry runs into the exponent by itself), held at the largest finite one; below, it is the count of
+// subnormal steps rounded half up. NaN gives a signed zero.
+template <bool kE5M2>
+__device__ __forceinline__ uint32_t fp8_code(h16 v) {
+    const uint32_t bits = __builtin_bit_cast(uint16_t, v), mag = bits & 0x7FFFu;
+    uint32_t code;
+    if constexpr (kE5M2) {
+        code = (mag + (mag < 0x400u ? 0x80u : 0x7Fu + ((mag >> 8) & 1u))) >> 8;
+        code = min(code, 0x7Bu);
+    } else {
+        const uint32_t low = (uint32_t)fmaf(fabsf((float)v), 512.0f, 0.5f);
+        code = (mag - 0x2000u + 0x3Fu + ((mag >> 7) & 1u)) >> 7;
+        code = mag < 0x2400u ? low : min(code, 0x7Eu);
+    }
+    return ((bits >> 8) & 0x80u) | (mag > 0x7C00u ? 0u : code);
+}
+
 template <int kFmt, bool kStream>
 __device__ __forceinline__ void store_values(void* store, size_t at, const Chunk& c) {      // eight, at element `at`
     if constexpr (kFmt == kFmtFp16) {
@@ -192,7 +215,7 @@ __device__ __forceinline__ void store_values(void* store, size_t at, const Chunk
         const h16x8 h = __builtin_bit_cast(h16x8, c);
         u32x2 w = {0u, 0u};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i >> 2] |= fp8_encode<kFmt == kFmtE5M2>((float)h[i]) << (8 * (i & 3));
+        for (int i = 0; i < 8; ++i) w[i >> 2] |= fp8_code<kFmt == kFmtE5M2>(h[i]) << (8 * (i & 3));
         u32x2* dst = reinterpret_cast<u32x2*>(static_cast<uint8_t*>(store) + at);
         if constexpr (kStream) __builtin_nontemporal_store(w, dst);
         else *dst = w;
@@ -202,16 +225,23 @@ __device__ __forceinline__ void store_values(void* store, size_t at, const Chunk
 constexpr int kAppendThreads = 1024;      // at most
 constexpr int kAppendRows = 8;            // rows a workgroup owns, at most
 
-template <int kHd, int kFmt, bool kStream>
+template <int kHd, int kFmt, bool kStream, bool kOneRow>
 __global__ __launch_bounds__(kAppendThreads) void append_rows(AppendArgs a, FreqTable freqs, int rows_per_wg) {
     constexpr int kItems = kHd / 16, kHalf = kHd / 2;
     __shared__ __attribute__((aligned(16))) float cs_cos[kAppendRows * kHalf], cs_sin[kAppendRows * kHalf];
     const int tid = (int)threadIdx.x;
-    const int row0 = (int)blockIdx.x * rows_per_wg, rows = min(rows_per_wg, a.rows - row0);
+    const int row0 = (int)blockIdx.x * (kOneRow ? 1 : rows_per_wg), rows = kOneRow ? 1 : min(rows_per_wg, a.rows - row0);
     const int per_row = (a.nq + 2 * a.nkv) * kItems, items = rows * per_row;
+    // Asked for before the tensors: memory returns in order, so the angles are computed while the tensors fly. Through the
+    // vector path, for which a zero that the compiler cannot see through stands in: as scalar loads, which it makes of a
+    // workgroup's one slot and position, 14449 rows of 28 + 4 heads take 51 us instead of 47.
+    int zero = 0;
+    asm volatile("" : "+v"(zero));
+    int my_pos = a.positions[row0 + min(tid / kHalf, rows - 1) + zero];
+    float my_freq = freqs.f[tid % kHalf];
     for (int base = 0; base < items; base += (int)blockDim.x) {       // one round unless a row has more than 1024 items
         const int item = min(base + tid, items - 1);
-        const int r = rows_per_wg == 1 ? 0 : item / per_row, in_row = item - r * per_row;
+        const int r = kOneRow ? 0 : item / per_row, in_row = item - r * per_row;
         const int head = in_row / kItems, c = in_row % kItems;
         const int kind = head < a.nq ? 0 : head < a.nq + a.nkv ? 1 : 2;
         const int h = kind == 0 ? head : kind == 1 ? head - a.nq : head - a.nq - a.nkv;
@@ -219,8 +249,8 @@ __global__ __launch_bounds__(kAppendThreads) void append_rows(AppendArgs a, Freq
         const h16* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + (row * (kind == 0 ? a.nq : a.nkv) + h) * kHd;
         const h16* bias = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
         const Chunk* p = reinterpret_cast<const Chunk*>(src) + c;
-        const Chunk lo = load_chunk_as<kStream>(p), hi = load_chunk_as<kStream>(p + kItems);
-        const int64_t slot = a.slots[row];
+        const int64_t slot = a.slots[row + zero];
+        const Chunk lo = load_chunk(p), hi = load_chunk(p + kItems);
         Chunk b0 = {}, b1 = {};
         if (bias) {
             const Chunk* bp = reinterpret_cast<const Chunk*>(bias + (size_t)h * kHd) + c;
@@ -228,9 +258,12 @@ __global__ __launch_bounds__(kAppendThreads) void append_rows(AppendArgs a, Freq
             b1 = load_chunk(bp + kItems);
         }
         if (base == 0) {
+            asm volatile("" : "+v"(my_pos), "+v"(my_freq));
             for (int i = tid; i < rows * kHalf; i += (int)blockDim.x) {
                 float s, cc;
-                sincosf((float)a.positions[row0 + i / kHalf] * freqs.f[i % kHalf], &s, &cc);
+                const bool mine = i == tid;
+                sincosf((float)(mine ? my_pos : a.positions[row0 + i / kHalf]) * (mine ? my_freq : freqs.f[i % kHalf]),
+                        &s, &cc);
                 cs_cos[i] = cc;
                 cs_sin[i] = s;
             }
@@ -376,8 +409,9 @@ vv_status_t vv_rope_kv_append_dev(const void* q, const void* k, const void* v, c
         const bool stream = vv::use_streaming(2u * (size_t)n_rows * (size_t)per_row * 32u);
 #define VV_APPEND(H, F)                                                                                \
     do {                                                                                               \
-        if (stream) vv::append_rows<H, vv::F, true><<<grid, threads, 0, st>>>(a, freqs, rows);         \
-        else        vv::append_rows<H, vv::F, false><<<grid, threads, 0, st>>>(a, freqs, rows);        \
+        if (rows > 1)    vv::append_rows<H, vv::F, false, false><<<grid, threads, 0, st>>>(a, freqs, rows); \
+        else if (stream) vv::append_rows<H, vv::F, true, true><<<grid, threads, 0, st>>>(a, freqs, rows);   \
+        else             vv::append_rows<H, vv::F, false, true><<<grid, threads, 0, st>>>(a, freqs, rows);  \
     } while (0)
         if (head_dim == 64)                       VV_APPEND(64, kFmtFp16);
         else if (!fp8)                            VV_APPEND(128, kFmtFp16);
