@@ -396,6 +396,28 @@ def test_attend_packed(fmt, nq, nkv):
     p.check(p.call())
 
 
+@pytest.mark.parametrize("fmt", [E4M3, E5M2])
+def test_attend_every_code(fmt):
+    """One position a sequence: the result is its value, for every finite code, exactly; and its key counts as that
+    value too: two positions whose keys differ in one channel's code alone share the weight as the codes say."""
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda")
+    value = codes.view(TORCH_FP8[fmt]).float()
+    finite = codes[torch.isfinite(value)]
+    n = finite.numel()
+    p = Pool([2] * n, 2, 1, 128, fmt=fmt, seed=21)
+    at = torch.from_numpy(np.stack([slots_of(t, 2) for t in p.tables])).cuda()
+    p.store[0][:] = 0
+    p.store[1][:] = 0
+    p.store[1][at[:, 0]] = finite[:, None, None]
+    out = p.call(lens=[1] * n)
+    want = finite.view(TORCH_FP8[fmt]).half()
+    assert torch.equal(out, want[:, None, None].expand(n, 2, 128))       # as numbers: +0 + -0 is +0
+    p.store[0][at[:, 0], 0, 37] = finite
+    p.q[:] = 0
+    p.q[:, :, 37] = 2.0 ** -6 if fmt == E4M3 else 2.0 ** -13          # scores of either sign, up to 1
+    p.check(p.call())
+
+
 @pytest.mark.parametrize("nq,nkv,hd", [(6, 3, 96), (4, 2, 256), (2, 1, 80), (4, 4, 1), (3, 1, 65)])
 def test_attend_other_head_dims(nq, nkv, hd):
     p = Pool(EDGES[:12], nq, nkv, hd, seed=hd)

@@ -3,8 +3,8 @@
 #include <algorithm>
 #ifndef VVD16
 #define VVD16 2
-#define VVD8 3
-#define VVD64 3
+#define VVD8 2
+#define VVD64 2
 #endif
 
 #include "attn_common.hpp"
@@ -83,6 +83,25 @@ struct Deal {
         return unit < longer ? unit / (q + 1) : r + (unit - longer) / max(q, 1);
     }
 };
+
+// Eight FP8 codes as the FP16 values they are, by the hardware's own conversion (a bit-by-bit widening of the 64 codes
+// a lane holds of sixteen positions was two thirds of the loop's vector instructions and bounded it).
+template <int kFmt>
+__device__ __forceinline__ h16x8 widen8(uint32_t a, uint32_t b) {
+    h16x8 out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = i < 2 ? a : b;
+        h16x2 v;
+        if constexpr (kFmt == kFmtE4M3) v = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)
+                                                  : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+        else v = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, 1.0f, true)
+                       : __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, 1.0f, false);
+        out[2 * i] = v[0];
+        out[2 * i + 1] = v[1];
+    }
+    return out;
+}
 
 // One page of a worker's run, ready to be fetched.
 struct __attribute__((aligned(16))) Item {
@@ -291,10 +310,8 @@ __global__ __launch_bounds__(kBatchThreads, VVOCC) void decode_batch(BatchArgs a
                             const Chunk codes = k_lds[wave][k_slot(position(c), 2 * j + s / 2)];
 #pragma unroll
                             for (int z = 0; z < 2; ++z) {
-                                Chunk w;
-                                widen4<kFmt>(codes.w[2 * z], w.w[0], w.w[1]);
-                                widen4<kFmt>(codes.w[2 * z + 1], w.w[2], w.w[3]);
-                                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, w), qf[s + z], sc, 0, 0, 0);
+                                const h16x8 keys = widen8<kFmt>(codes.w[2 * z], codes.w[2 * z + 1]);
+                                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, qf[s + z], sc, 0, 0, 0);
                             }
                         }
                     }
@@ -320,15 +337,8 @@ __global__ __launch_bounds__(kBatchThreads, VVOCC) void decode_batch(BatchArgs a
                             for (int odd = 0; odd < 2; ++odd) {
                                 const bool own = odd == 0 ? c < 8 : c >= 8;
                                 const uint32_t w0 = own ? keep[0] : got[0], w1 = own ? keep[1] : got[1];
-                                Chunk w = {};
-                                if constexpr (kFmt == kFmtFp16) {
-                                    w.w[0] = w0;
-                                    w.w[1] = w1;
-                                } else {
-                                    widen4<kFmt>(w0, w.w[0], w.w[1]);
-                                    widen4<kFmt>(w1, w.w[2], w.w[3]);
-                                }
-                                v4[2 * x + odd] = __builtin_bit_cast(h16x8, w);
+                                if constexpr (kFmt == kFmtFp16) v4[2 * x + odd] = __builtin_bit_cast(h16x8, Chunk{{w0, w1, 0, 0}});
+                                else v4[2 * x + odd] = widen8<kFmt>(w0, w1);
                             }
                         }
                     }
