@@ -93,6 +93,7 @@ def test_attend_refusals():
         assert attend_call(**{name: 0}) == dev.VV_ERR_INVALID_ARG
     assert attend_call(max_pages=1 << 25) == dev.VV_ERR_UNSUPPORTED             # positions past 32 bits
     assert attend_call(n_seqs=1 << 16, max_pages=1 << 15) == dev.VV_ERR_UNSUPPORTED
+    assert attend_call(n_seqs=(1 << 21) + 1, max_pages=1) == dev.VV_ERR_UNSUPPORTED     # rows past a launch
     need = dev.vv_attn_decode_batch_scratch_bytes(3, 4, 2, 128)
     assert attend_call(scratch_bytes=need - 1) == dev.VV_ERR_INVALID_ARG
     assert attend_call(scratch=P + 4) == dev.VV_ERR_INVALID_ARG
@@ -103,7 +104,7 @@ def test_scratch_grows_with_the_sequences_by_their_count_alone():
     assert size(0, 4, 2, 128) == size(3, 4, 3, 128) == size(3, 0, 2, 128) == size(3, 4, 2, 0) == 0
     one = size(1, 28, 4, 128)
     assert 0 < one < 64 << 20
-    assert one <= size(100, 28, 4, 128) <= one + 101 * 4 + 256
+    assert one <= size(100, 28, 4, 128) <= one + 100 * 4 * 8 + 256
     assert size(1, 40, 2, 128) >= size(1, 20, 2, 128)
 
 

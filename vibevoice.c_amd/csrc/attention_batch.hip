@@ -1,11 +1,36 @@
 // Decode attention of many sequences over one paged pool: one query row per sequence and head, each sequence behind its
 // own row of page ids and of its own length, the lengths on the device.
+//
+//   out[i, h] = sum_t p_t V[t] / sum_t p_t,  p_t = exp(q[i, h] . K[t] / sqrt(hd)),  t < lens[i]
+//
+// Bound by the bytes of the cache, which are read once: 4 hd lens[i] a KV head (FP16) for 4 hd lens[i] flops a query
+// head. So what counts is that the memory system has enough requests from the first microsecond to the last, whatever
+// the lengths are:
+//   deal     The work is the list of units (sequence, KV head, page) in that order, cut into 512 runs of equal
+//            length, one for each workgroup ("worker"): two workgroups of four waves for each compute unit, all resident
+//            at once. Nothing is sized by the longest sequence and nothing depends on the host knowing a length. Each
+//            worker finds its run by a prefix sum over the lengths (4 bytes a sequence), looks its page ids up into LDS
+//            256 at a time, and then only reads pages. A unit is 16 KB of K and 16 KB of V at 128 channels: fewer
+//            positions would cut rows into more partial states than they save in balance. More workers, 768 or 1024,
+//            with or without more of them resident, or a last quarter of the work dealt to 512 smaller ones, are no
+//            faster on long caches (146 to 154 us against 146 at 32 x 13400 positions) and up to 45 % slower
+//            on short ones, through their partial states.
+//   stream   Of a page each wave takes sixteen positions. Its loads are buffer loads bounded by the positions in use:
+//            what lies past them (or behind a bad page id) is not read and comes as zeros, and since every item, an
+//            empty one behind the last too, issues the same loads, the compiler can count them: the next two items'
+//            loads are in flight while one is computed (one: the same to 3 % slower; three: 10 to 25 % slower).
+//            They are non-temporal (a plain read of 512 MB runs at 6.7 TB/s so, at 5.9 without).
+//   products S = K Q^T (16x16x32, sixteen positions by up to sixteen query heads of the group), the softmax online per
+//            head in FP32, O^T = V^T P^T (16x16x16). V's share of the operand is picked from the registers; K takes a
+//            turn through the wave's own LDS (struct Block).
+//   join     Where a run ends a row (sequence, KV head) the four waves' states meet in LDS. A row that lies
+//            wholly inside a worker is finished there; otherwise each worker leaves (sum of p V, maximum, sum of p) in
+//            `parts`, and a second launch folds them in the order of their pages.
+// Measured at 28 + 4 heads of 128 (both launches, cache cold, three caches in turn): 1 x 14449 positions 14.4 us,
+// 8 x 2048 14.5, 24 of 0 .. 14449 65.4 us (5.4 TB/s), 32 of 12345 .. 14449 146.5 us (6.0 TB/s, 94 % of what a plain
+// read of 256-byte vectors reaches); 64 of 6001 .. 8192 in E4M3 84.6 us (5.5 TB/s). What is left below 100 MB is latency: 3.2
+// us until a worker's first loads go out (lengths, page ids), 3 until they are back, and 4.4 for the second launch.
 #include <algorithm>
-#ifndef VVD16
-#define VVD16 2
-#define VVD8 2
-#define VVD64 2
-#endif
 
 #include "attn_common.hpp"
 
@@ -14,16 +39,14 @@ namespace {
 
 constexpr int kBatchThreads = 256;
 constexpr int kBatchWaves = kBatchThreads / kWave;
-#ifndef VVW
-#define VVW 512
-#define VVOCC 2
-#endif
-constexpr int kWorkers = VVW;                // workgroups the pages are dealt to: two for each of 256 compute units
+constexpr int kWorkers = 512;
 constexpr int kSliceHeads = 16;              // query heads of a group that one workgroup takes: a matrix tile's columns
 constexpr int kSeqChunk = 1024;              // sequences whose lengths a workgroup holds at a time
-// A probability is formed on the scale 2^kLift of the row's maximum, so that it leaves FP16's normal range only 2^24
-// below that; the factor is in the sum of the row too and cancels.
+// A probability is rounded to FP16 for the matrix product (half a step, 2^-11 of it; the row's sum takes it unrounded).
+// It is formed on the scale 2^kLift of the row's maximum, so that it leaves FP16's normal range only 2^24 below that;
+// the factor is in the row's sum too and cancels.
 constexpr float kLift = 10.0f;
+constexpr int kDepth = 2;                    // items whose loads are in flight while one is computed
 constexpr int kItems = 256;                  // pages whose work a workgroup holds at a time
 
 struct Row {                                 // a row of the work: (sequence, KV head)
@@ -138,8 +161,8 @@ __device__ __forceinline__ Chunk load16(__amdgpu_buffer_rsrc_t r, uint32_t at) {
     return __builtin_bit_cast(Chunk, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, kNonTemporal));
 }
 
-template <int kHd, int kFmt, int kDepth>
-__global__ __launch_bounds__(kBatchThreads, VVOCC) void decode_batch(BatchArgs a) {
+template <int kHd, int kFmt>
+__global__ __launch_bounds__(kBatchThreads, 2) void decode_batch(BatchArgs a) {
     typedef Block<kHd, kFmt> B;
     constexpr int kSteps = kHd / 32;                       // 32-channel steps of the score product
     constexpr bool kNarrow = B::kRow == 128;
@@ -416,9 +439,10 @@ __global__ __launch_bounds__(kBatchThreads, VVOCC) void decode_batch(BatchArgs a
                             l_all = fmaf(l_lds[w][h], f, l_all);
                         }
                         if (whole) {
+                            const float inv = l_all == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(l_all);
                             h16* to = a.out + ((size_t)it.seq * a.n_q_heads + head0 + h) * kHd + ch;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) to[r] = to_half(l_all == 0.0f ? 0.0f : ov[r] / l_all);
+                            for (int r = 0; r < 4; ++r) to[r] = to_half(ov[r] * inv);
                         } else {
                             float* rec = dst + (size_t)h * part_floats(kHd);
                             *reinterpret_cast<f32x4*>(rec + ch) = ov;
@@ -515,8 +539,9 @@ __global__ void decode_batch_merge(BatchArgs a, int slices, int heads_per_wg) {
     }
     const int seq = row / a.n_kv_heads, kvh = row - seq * a.n_kv_heads;
     h16* dst = a.out + ((size_t)seq * a.n_q_heads + kvh * group + in_group) * kHd + 4 * quad;
+    const float inv = l == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(l);      // 1 ulp of FP32
 #pragma unroll
-    for (int r = 0; r < 4; ++r) dst[r] = to_half(l == 0.0f ? 0.0f : o[r] / l);
+    for (int r = 0; r < 4; ++r) dst[r] = to_half(o[r] * inv);
 }
 
 // Any head_dim <= 256, any alignment, FP16: a wave per (sequence, head) walks the sequence's keys.
@@ -567,9 +592,9 @@ inline size_t row_bytes(int n_seqs, int n_kv_heads) {
     return ((size_t)n_seqs * n_kv_heads * sizeof(Row) + 255) & ~(size_t)255;
 }
 
-template <int kHd, int kFmt, int kDepth>
+template <int kHd, int kFmt>
 void launch(const BatchArgs& a, int slices, hipStream_t st) {
-    decode_batch<kHd, kFmt, kDepth><<<dim3(kWorkers, (unsigned)slices), kBatchThreads, 0, st>>>(a);
+    decode_batch<kHd, kFmt><<<dim3(kWorkers, (unsigned)slices), kBatchThreads, 0, st>>>(a);
 }
 
 template <int kHd>
@@ -610,8 +635,8 @@ vv_status_t vv_attn_decode_batch(int backend, const void* q, const vv_kv_view_t*
     if (n_q_heads <= 0 || n_q_heads > 65535 || kv->n_kv_heads <= 0 || n_q_heads % kv->n_kv_heads || kv->head_dim <= 0 || kv->head_dim > 256)
         return VV_ERR_UNSUPPORTED;
     if (max_pages <= 0 || n_pages <= 0) return VV_ERR_INVALID_ARG;
-    // the list of (sequence, KV head, page) is counted in 32 bits
-    if ((int64_t)max_pages * vv::kPage > INT32_MAX || (int64_t)n_seqs * max_pages * kv->n_kv_heads > INT32_MAX - vv::kWorkers)
+    // the list of (sequence, KV head, page) is counted in 32 bits, and a launch has a workgroup per row of it
+    if ((int64_t)n_seqs * kv->n_kv_heads > (1 << 22) || (int64_t)max_pages * vv::kPage > INT32_MAX || (int64_t)n_seqs * max_pages * kv->n_kv_heads > INT32_MAX - vv::kWorkers)
         return VV_ERR_UNSUPPORTED;
     vv::BatchArgs a = {static_cast<const vv::h16*>(q), kv->k, kv->v, kv->page_table, cache_lens,
                        static_cast<vv::h16*>(out), nullptr, nullptr, n_q_heads, kv->n_kv_heads, n_seqs, max_pages,
@@ -626,10 +651,10 @@ vv_status_t vv_attn_decode_batch(int backend, const void* q, const vv_kv_view_t*
         a.rows = static_cast<vv::Row*>(scratch);
         a.parts = reinterpret_cast<float*>(static_cast<char*>(scratch) + vv::row_bytes(n_seqs, kv->n_kv_heads));
         const int group = n_q_heads / kv->n_kv_heads, slices = (group + vv::kSliceHeads - 1) / vv::kSliceHeads;
-        if (kv->head_dim == 64) vv::launch<64, vv::kFmtFp16, VVD64>(a, slices, st);
-        else if (kv->format == vv::kFmtFp16) vv::launch<128, vv::kFmtFp16, VVD16>(a, slices, st);
-        else if (kv->format == vv::kFmtE4M3) vv::launch<128, vv::kFmtE4M3, VVD8>(a, slices, st);
-        else vv::launch<128, vv::kFmtE5M2, VVD8>(a, slices, st);
+        if (kv->head_dim == 64) vv::launch<64, vv::kFmtFp16>(a, slices, st);
+        else if (kv->format == vv::kFmtFp16) vv::launch<128, vv::kFmtFp16>(a, slices, st);
+        else if (kv->format == vv::kFmtE4M3) vv::launch<128, vv::kFmtE4M3>(a, slices, st);
+        else vv::launch<128, vv::kFmtE5M2>(a, slices, st);
         if (hipGetLastError() != hipSuccess) return VV_ERR_CUDA_LAUNCH;
         if (kv->head_dim == 64) vv::launch_merge<64>(a, slices, st);
         else vv::launch_merge<128>(a, slices, st);
