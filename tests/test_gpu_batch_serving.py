@@ -432,7 +432,8 @@ def test_attend_unaligned_query():
 
 
 @pytest.mark.parametrize("lens", [[14449], [5000, 1, 9000, 64], [64] * 300, [1] * 1500, list(range(700)),
-                                  [0] * 1100 + [77]])
+                                  [0] * 1100 + [77], [9000] + [60] * 39,
+                                  [60] * 150 + [20000] + [60] * 149])
 def test_attend_many_and_long(lens):
     """One long sequence over all workgroups, more sequences than threads, than workgroups, mostly empty ones."""
     p = Pool(lens, 4, 2, 128, seed=len(lens))

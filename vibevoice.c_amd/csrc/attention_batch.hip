@@ -468,22 +468,21 @@ __global__ __launch_bounds__(kBatchThreads, 2) void decode_batch(BatchArgs a) {
     }
 }
 
-// Folds the partial states of the rows that several workers share, in the order of their pages. A thread holds four
-// channels of one head over every kGroups-th part; the groups' states meet in LDS.
-template <int kHd, int kGroups>
-__global__ void decode_batch_merge(BatchArgs a, int slices, int heads_per_wg) {
+// Folds the partial states of the rows that several workers share, in the order of their pages. A workgroup has kHeads
+// heads of a row; a thread holds four channels of one of them over every kGroups-th part, and the groups' states meet
+// in LDS.
+template <int kHd, int kHeads, int kGroups>
+__global__ __launch_bounds__(kHd / 4 * kHeads * kGroups) void decode_batch_merge(BatchArgs a, int slices) {
     constexpr int kQuads = kHd / 4;
-    __shared__ float s_m[kGroups], s_l[kGroups];
-    __shared__ __attribute__((aligned(16))) float s_o[kGroups > 1 ? kGroups * kHd : 1];
+    __shared__ float s_m[kGroups][kHeads], s_l[kGroups][kHeads];
+    __shared__ __attribute__((aligned(16))) float s_o[kGroups > 1 ? kGroups * kHeads * kHd : 1];
     const int group = a.n_q_heads / a.n_kv_heads;
     const int row = (int)blockIdx.x, per = min(group, kSliceHeads);
     const Row at = a.rows[row];
     if (at.first == at.last) return;                                     // that worker wrote the output
-    const int quad = (int)threadIdx.x % kQuads;
-    const int rest = (int)threadIdx.x / kQuads;
-    const int grp = kGroups > 1 ? rest : 0;
-    const int in_group = (int)blockIdx.y * heads_per_wg + (kGroups > 1 ? 0 : rest);
-    if (kGroups == 1 && (rest >= heads_per_wg || in_group >= group)) return;
+    const int quad = (int)threadIdx.x % kQuads, local = (int)threadIdx.x / kQuads % kHeads;
+    const int grp = (int)threadIdx.x / (kQuads * kHeads);
+    const int want = (int)blockIdx.y * kHeads + local, in_group = min(want, group - 1);
     const int slice = in_group / kSliceHeads, h = in_group - slice * kSliceHeads;
     auto part = [&](int w) {
         return a.parts + ((((size_t)w * 2 + (w == at.first ? 1 : 0)) * slices + slice) * per + h) * part_floats(kHd);
@@ -520,23 +519,24 @@ __global__ void decode_batch_merge(BatchArgs a, int slices, int heads_per_wg) {
         m = m_new;
     }
     if constexpr (kGroups > 1) {
-        if (quad == 0) { s_m[grp] = m; s_l[grp] = l; }
-        *reinterpret_cast<f32x4*>(&s_o[grp * kHd + 4 * quad]) = o;
+        if (quad == 0) { s_m[grp][local] = m; s_l[grp][local] = l; }
+        *reinterpret_cast<f32x4*>(&s_o[(grp * kHeads + local) * kHd + 4 * quad]) = o;
         __syncthreads();
         if (grp > 0) return;
-        for (int g = 0; g < kGroups; ++g) m = fmaxf(m, s_m[g]);
+        for (int g = 0; g < kGroups; ++g) m = fmaxf(m, s_m[g][local]);
         const float m_use = m == -INFINITY ? 0.0f : m;
         o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         l = 0.0f;
 #pragma unroll 8
         for (int g = 0; g < kGroups; ++g) {
-            const float f = exp2_fast(s_m[g] - m_use);
-            const f32x4 og = *reinterpret_cast<const f32x4*>(&s_o[g * kHd + 4 * quad]);
-            l = fmaf(s_l[g], f, l);
+            const float f = exp2_fast(s_m[g][local] - m_use);
+            const f32x4 og = *reinterpret_cast<const f32x4*>(&s_o[(g * kHeads + local) * kHd + 4 * quad]);
+            l = fmaf(s_l[g][local], f, l);
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = fmaf(og[r], f, o[r]);
         }
     }
+    if (want >= group) return;
     const int seq = row / a.n_kv_heads, kvh = row - seq * a.n_kv_heads;
     h16* dst = a.out + ((size_t)seq * a.n_q_heads + kvh * group + in_group) * kHd + 4 * quad;
     const float inv = l == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(l);      // 1 ulp of FP32
@@ -597,18 +597,25 @@ void launch(const BatchArgs& a, int slices, hipStream_t st) {
     decode_batch<kHd, kFmt><<<dim3(kWorkers, (unsigned)slices), kBatchThreads, 0, st>>>(a);
 }
 
+template <int kHd, int kHeads, int kThreads>
+void launch_merge_of(const BatchArgs& a, int slices, hipStream_t st) {
+    const dim3 grid((unsigned)(a.n_seqs * a.n_kv_heads), (unsigned)((a.n_q_heads / a.n_kv_heads - 1) / kHeads + 1));
+    decode_batch_merge<kHd, kHeads, kThreads * 4 / (kHd * kHeads)><<<grid, kThreads, 0, st>>>(a, slices);
+}
+// The fewer rows, the more parts a row can have, and the more threads are put to one; but a workgroup costs its launch
+// also where a row has nothing to fold, which is what many rows mostly have. Measured (both launches) at 28 + 4 heads with
+// one head of 1024 threads / one of 256 / two of 256 / four of 256 / eight of 256 a workgroup:
+//   one sequence of 14449 positions and 39 of 60 (160 rows)    - / 16.9 / 19.0 / 23.3 / 30.8 us
+//   one of 32000 and 249 of 60 (1000 rows)                     - / 31.2 / -    / 33.9 / 39.7
+//   128 of 50 .. 150 (512 rows)                                - / 15.3 / 15.0 / 14.9 / 14.3
+//   1000 of 64 (4000 rows)                                     -  / -  / -  / 35.7 / 34.7
+//   one of 14449 (4 rows): 14.4 with one head of 1024 threads, 15.0 with one of 256.
 template <int kHd>
 void launch_merge(const BatchArgs& a, int slices, hipStream_t st) {
-    const int rows = a.n_seqs * a.n_kv_heads, group = a.n_q_heads / a.n_kv_heads;
-    constexpr int kMany = 1024 / (kHd / 4);
-    if (rows <= 32) {
-        decode_batch_merge<kHd, kMany><<<dim3((unsigned)rows, (unsigned)group), 1024, 0, st>>>(a, slices, 1);
-    } else {
-        const int heads = std::min(group, 8);
-        const unsigned threads = (unsigned)(heads * (kHd / 4) + kWave - 1) / kWave * kWave;
-        decode_batch_merge<kHd, 1><<<dim3((unsigned)rows, (unsigned)((group + heads - 1) / heads)), threads, 0, st>>>(
-            a, slices, heads);
-    }
+    const int rows = a.n_seqs * a.n_kv_heads;
+    if (rows <= 32) launch_merge_of<kHd, 1, 1024>(a, slices, st);
+    else if (rows <= 512) launch_merge_of<kHd, 2, 256>(a, slices, st);
+    else launch_merge_of<kHd, 4, 256>(a, slices, st);
 }
 
 }  // namespace
