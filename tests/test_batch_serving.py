@@ -89,6 +89,7 @@ def test_attend_refusals():
     assert attend_call({"head_dim": 0}) == dev.VV_ERR_UNSUPPORTED
     assert attend_call({"n_kv_heads": 3}) == dev.VV_ERR_UNSUPPORTED
     assert attend_call(n_q_heads=0) == dev.VV_ERR_UNSUPPORTED
+    assert attend_call(n_q_heads=16386) == dev.VV_ERR_UNSUPPORTED
     for name in ("max_pages", "n_pages"):
         assert attend_call(**{name: 0}) == dev.VV_ERR_INVALID_ARG
     assert attend_call(max_pages=1 << 25) == dev.VV_ERR_UNSUPPORTED             # positions past 32 bits

@@ -394,6 +394,15 @@ def test_attend_edges(nq, nkv, hd):
 def test_attend_packed(fmt, nq, nkv):
     p = Pool(EDGES, nq, nkv, 128, fmt=fmt, seed=nq + fmt)
     p.check(p.call())
+    # a bad page in either place of a pair, and both
+    tables = p.tables.copy()
+    tables[15, 1] = -1
+    tables[16, [2, 3, 6]] = p.n_pages
+    drop = {15: [*range(64, 128)], 16: [*range(128, 256), *range(384, 448)]}
+
+    def values(i):
+        return [np.delete(x, drop[i], 0) for x in p.values(i)]
+    p.check(p.call(tables=tables), rows=[15, 16], values=values)
 
 
 @pytest.mark.parametrize("fmt", [E4M3, E5M2])
@@ -433,7 +442,8 @@ def test_attend_unaligned_query():
 
 @pytest.mark.parametrize("lens", [[14449], [5000, 1, 9000, 64], [64] * 300, [1] * 1500, list(range(700)),
                                   [0] * 1100 + [77], [9000] + [60] * 39,
-                                  [60] * 150 + [20000] + [60] * 149])
+                                  [60] * 150 + [20000] + [60] * 149,
+                                  [3] * 300 + [6000] + [0] * 300])
 def test_attend_many_and_long(lens):
     """One long sequence over all workgroups, more sequences than threads, than workgroups, mostly empty ones."""
     p = Pool(lens, 4, 2, 128, seed=len(lens))
@@ -504,6 +514,18 @@ def test_attend_infinities_and_nan(hd):
     keep = np.delete(np.arange(65), 10)
     want, mag = attend(p.q[1, 2:].float().cpu().numpy().astype(np.float64), k[keep, 1:], v[keep, 1:])
     assert (np.abs(out[1, 2:] - want) <= attend_bound(want, mag, 65, np.abs(v).max())).all()
+
+
+def test_attend_nan_query():
+    """A query that is NaN gives NaN for its head, short rows and rows that many workgroups share, and for no other."""
+    p = Pool([5000, 70, 0, 3000], 4, 2, 128, seed=22)
+    p.q[0, 1, 5] = float("nan")
+    p.q[1, 2, 0] = float("nan")
+    out = p.call()
+    bad = torch.isnan(out).all(-1).cpu().numpy()
+    assert bad.tolist() == [[False, True, False, False], [False, False, True, False], [False] * 4, [False] * 4]
+    assert torch.isfinite(out[torch.from_numpy(~bad).cuda()]).all()
+    p.check(out, rows=[3])
 
 
 @pytest.mark.parametrize("scale", [1e-3, 30.0])

@@ -27,7 +27,7 @@
 //            wholly inside a worker is finished there; otherwise each worker leaves (sum of p V, maximum, sum of p) in
 //            `parts`, and a second launch folds them in the order of their pages.
 // Measured at 28 + 4 heads of 128 (both launches, cache cold, three caches in turn): 1 x 14449 positions 14.4 us,
-// 8 x 2048 14.5, 24 of 0 .. 14449 65.4 us (5.4 TB/s), 32 of 12345 .. 14449 146.5 us (6.0 TB/s, 94 % of what a plain
+// 8 x 2048 13.6, 24 of 0 .. 14449 64.6 us (5.5 TB/s), 32 of 12345 .. 14449 146.5 us (6.0 TB/s, 94 % of what a plain
 // read of 256-byte vectors reaches); 64 of 6001 .. 8192 in E4M3 84.6 us (5.5 TB/s). What is left below 100 MB is latency: 3.2
 // us until a worker's first loads go out (lengths, page ids), 3 until they are back, and 4.4 for the second launch.
 #include <algorithm>
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(kHd / 4 * kHeads * kGroups) void decode_batch_merge
     };
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 4;
     for (int w0 = at.first + grp; w0 <= at.last; w0 += kAhead * kGroups) {
         f32x4 ov[kAhead];
         float mv[kAhead], lv[kAhead];
@@ -498,8 +498,8 @@ __global__ __launch_bounds__(kHd / 4 * kHeads * kGroups) void decode_batch_merge
             const int w = w0 + i * kGroups;
             const float* p = part(min(w, at.last));
             ov[i] = *reinterpret_cast<const f32x4*>(p + 4 * quad);
-            mv[i] = w <= at.last ? p[kHd] : -INFINITY;
-            lv[i] = p[kHd + 1];
+            mv[i] = p[kHd];
+            lv[i] = w <= at.last ? p[kHd + 1] : 0.0f;      // (behind the last part: the last once more, unused)
         }
         float m_new = m;
 #pragma unroll
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(kHd / 4 * kHeads * kGroups) void decode_batch_merge
         l *= keep;
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            if (mv[i] == -INFINITY) continue;              // nothing seen there: no part of the sums, whatever it holds
+            if (lv[i] == 0.0f) continue;                   // nothing seen there (a part that saw only NaN has NaN here)
             const float f = exp2_fast(mv[i] - m_use);
             l = fmaf(lv[i], f, l);
 #pragma unroll
@@ -604,17 +604,18 @@ void launch_merge_of(const BatchArgs& a, int slices, hipStream_t st) {
 }
 // The fewer rows, the more parts a row can have, and the more threads are put to one; but a workgroup costs its launch
 // also where a row has nothing to fold, which is what many rows mostly have. Measured (both launches) at 28 + 4 heads with
-// one head of 1024 threads / one of 256 / two of 256 / four of 256 / eight of 256 a workgroup:
-//   one sequence of 14449 positions and 39 of 60 (160 rows)    - / 16.9 / 19.0 / 23.3 / 30.8 us
-//   one of 32000 and 249 of 60 (1000 rows)                     - / 31.2 / -    / 33.9 / 39.7
-//   128 of 50 .. 150 (512 rows)                                - / 15.3 / 15.0 / 14.9 / 14.3
-//   1000 of 64 (4000 rows)                                     -  / -  / -  / 35.7 / 34.7
-//   one of 14449 (4 rows): 14.4 with one head of 1024 threads, 15.0 with one of 256.
+// one head of 1024 threads / one of 256 / two of 256 / four of 256 / eight of 256 a workgroup, in us:
+//   one sequence of 14449 positions (4 rows)             14.5 / 16.0 / 19.7 / 27.7 / 43.4
+//   8 of 2048 (32 rows)                                  14.4 / 13.6 / 13.5 / 14.3 / 15.6
+//   one of 14449 and 39 of 60 (160 rows)                  -   / 17.7 / 20.5 / 25.9 / 35.9
+//   128 of 50 .. 150 (512 rows)                           -   / 14.5 / 14.5 / 14.4 / 14.0
+//   one of 32000 and 249 of 60 (1000 rows)                -   / 30.7 / 32.3 / 35.8 / 43.3
+//   1000 of 64 (4000 rows)                                -   / 39.7 / 37.2 / 35.7 / 34.9
 template <int kHd>
 void launch_merge(const BatchArgs& a, int slices, hipStream_t st) {
     const int rows = a.n_seqs * a.n_kv_heads;
-    if (rows <= 32) launch_merge_of<kHd, 1, 1024>(a, slices, st);
-    else if (rows <= 512) launch_merge_of<kHd, 2, 256>(a, slices, st);
+    if (rows <= 16) launch_merge_of<kHd, 1, 1024>(a, slices, st);
+    else if (rows <= 1024) launch_merge_of<kHd, 1, 256>(a, slices, st);
     else launch_merge_of<kHd, 4, 256>(a, slices, st);
 }
 
@@ -639,7 +640,7 @@ vv_status_t vv_attn_decode_batch(int backend, const void* q, const vv_kv_view_t*
     if (!kv->k || !kv->v || !kv->page_table) return VV_ERR_NULL_PTR;
     const bool fp8 = kv->format == vv::kFmtE4M3 || kv->format == vv::kFmtE5M2;
     if (kv->format != vv::kFmtFp16 && !(fp8 && kv->head_dim == 128)) return VV_ERR_UNSUPPORTED;
-    if (n_q_heads <= 0 || n_q_heads > 65535 || kv->n_kv_heads <= 0 || n_q_heads % kv->n_kv_heads || kv->head_dim <= 0 || kv->head_dim > 256)
+    if (n_q_heads <= 0 || n_q_heads > (1 << 14) || kv->n_kv_heads <= 0 || n_q_heads % kv->n_kv_heads || kv->head_dim <= 0 || kv->head_dim > 256)
         return VV_ERR_UNSUPPORTED;
     if (max_pages <= 0 || n_pages <= 0) return VV_ERR_INVALID_ARG;
     // the list of (sequence, KV head, page) is counted in 32 bits, and a launch has a workgroup per row of it
