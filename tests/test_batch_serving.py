@@ -50,6 +50,8 @@ def test_plan_refusals():
     assert plan_call(max_rows=-1) == dev.VV_ERR_INVALID_ARG
     assert plan_call(lens_out=P) == dev.VV_ERR_INVALID_ARG            # the lengths over the request they follow from
     assert plan_call(counts=P) == dev.VV_ERR_INVALID_ARG              # the counts over the number of free pages
+    assert plan_call(counts=P + 192) == dev.VV_ERR_INVALID_ARG        # or over what is left of them
+    assert plan_call(max_rows=(1 << 30) + 1) == dev.VV_ERR_UNSUPPORTED
 
 
 @pytest.mark.parametrize("name", ["q", "k", "v", "positions", "slots", "q_out", "k_store", "v_store"])

@@ -348,11 +348,14 @@ class Pool:
         x = [s[at] if self.fmt == FP16 else s[at].view(TORCH_FP8[self.fmt]) for s in self.store]
         return [t.float().cpu().numpy().astype(np.float64) for t in x]
 
-    def call(self, lens=None, tables=None, stream_=None, q=None, n=None, scratch_fill=0xFF):
+    def call(self, lens=None, tables=None, stream_=None, q=None, n=None, scratch_fill=0xFF, in_place=False):
         n = len(self.lens) if n is None else n
         q = self.q if q is None else q
         d_lens, d_tables = ints(self.lens if lens is None else lens), ints(self.tables if tables is None else tables)
         out = torch.full((n + 1, self.nq, self.hd), float("nan"), dtype=torch.float16, device="cuda")
+        if in_place:
+            out[:n] = q
+            q = out
         size = dev.vv_attn_decode_batch_scratch_bytes(n, self.nq, self.nkv, self.hd)
         scratch = torch.full((size + 64,), scratch_fill, dtype=torch.uint8, device="cuda")      # NaN unless written
         view = dev.KvView(k=self.store[0].data_ptr(), v=self.store[1].data_ptr(), k_meta=None, v_meta=None,
@@ -387,6 +390,7 @@ def test_attend_edges(nq, nkv, hd):
     p.check(out)
     assert (out[1] == 0).all() and (out[14] == 0).all()
     assert np.array_equal(raw(p.call(scratch_fill=0)), raw(out)), "another answer the second time"
+    assert np.array_equal(raw(p.call(in_place=True)), raw(out)), "another answer over the query"
 
 
 @pytest.mark.parametrize("fmt", [E4M3, E5M2])
@@ -449,6 +453,7 @@ def test_attend_many_and_long(lens):
     p = Pool(lens, 4, 2, 128, seed=len(lens))
     out = p.call()
     p.check(out, rows=sorted(set(range(0, len(lens), max(1, len(lens) // 12))) | {len(lens) - 1}))
+    assert np.array_equal(raw(p.call(in_place=True)), raw(out)), "another answer over the query"
     empty = [i for i, n in enumerate(lens) if n == 0]
     assert (out[empty] == 0).all()
 

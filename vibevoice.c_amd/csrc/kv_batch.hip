@@ -360,8 +360,9 @@ vv_status_t vv_kv_page_plan_dev(const int* new_lens, const int* cache_lens, int 
     if (!new_lens || !cache_lens || !page_tables || !free_pages || !n_free || !lens_out || !row_starts || !counts)
         return VV_ERR_NULL_PTR;
     if (max_pages <= 0 || max_rows < 0) return VV_ERR_INVALID_ARG;
+    if (max_rows > (1 << 30)) return VV_ERR_UNSUPPORTED;           // a saturated row count is past every row then
     if (max_rows > 0 && (!positions || !slots)) return VV_ERR_NULL_PTR;
-    if (lens_out == new_lens || counts == n_free) return VV_ERR_INVALID_ARG;
+    if (lens_out == new_lens || counts == n_free || counts == n_free_out) return VV_ERR_INVALID_ARG;
     vv::PlanArgs a = {new_lens, cache_lens, page_tables, free_pages, n_free, lens_out, row_starts, positions, slots,
                       n_free_out, counts, n_seqs, max_pages, max_rows, max_rows};
     const int threads = n_seqs <= 64 && max_rows <= 64 ? 64 : n_seqs <= 256 ? 256 : vv::kPlanThreads;
