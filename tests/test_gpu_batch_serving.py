@@ -717,3 +717,50 @@ def test_serving_loop(fmt, captured):
     assert refused > 0
     if captured:
         dev.vv_dev_graph_destroy(graph)
+
+
+@pytest.mark.parametrize("fmt", [FP16, E5M2])
+def test_step_with_a_prompt(fmt):
+    """Decoding requests first, a prompt's chunk behind them: one plan, one append, batched attention for the former and
+    the paged prefill for the latter, all on one pool."""
+    nq, nkv, hd, max_pages, theta = 8, 2, 128, 4, 1e6
+    p = Pool([100, 63, 1, 200, 90], nq, nkv, hd, fmt=fmt, seed=31, max_pages=max_pages, spare=8)
+    n_dec, chunk = 4, 70
+    held = [p.values(i) for i in range(5)]
+    free = np.setdiff1d(np.arange(p.n_pages), p.tables)
+    new, n_free = [1] * n_dec + [chunk], len(free)
+    rows = sum(new)
+    x = [to_dev(oracle.normal_f16((rows, n, hd), 70 + i)) for i, n in enumerate((nq, nkv, nkv))]
+    d = dict(new=ints(new), lens=ints(p.lens), tables=ints(p.tables), free=ints(free), n_free=ints([n_free]),
+             starts=ints([0] * 6), pos=ints([0] * rows), slots=ints([0] * rows, torch.int64), counts=ints([0] * 3))
+    at = {k: t.data_ptr() for k, t in d.items()}
+    ok(dev.vv_kv_page_plan_dev(at["new"], at["lens"], 5, at["tables"], max_pages, at["free"], at["n_free"], at["lens"],
+                               at["starts"], at["pos"], at["slots"], rows, at["n_free"], at["counts"], stream()))
+    ok(dev.vv_rope_kv_append_dev(*(t.data_ptr() for t in x), None, None, None, at["pos"], at["slots"], x[0].data_ptr(),
+                                 p.store[0].data_ptr(), p.store[1].data_ptr(), rows, nq, nkv, hd, p.n_pages, fmt, theta,
+                                 stream()))
+    view = dev.KvView(k=p.store[0].data_ptr(), v=p.store[1].data_ptr(), k_meta=None, v_meta=None,
+                      page_table=at["tables"], format=fmt, n_kv_heads=nkv, head_dim=hd)
+    size = dev.vv_attn_decode_batch_scratch_bytes(n_dec, nq, nkv, hd)
+    scratch, out = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.full_like(x[0], float("nan"))
+    ok(dev.vv_attn_decode_batch(2, x[0].data_ptr(), C.addressof(view), out.data_ptr(), nq, n_dec, at["lens"], max_pages,
+                                p.n_pages, scratch.data_ptr(), size, stream()))
+    one = dev.KvView(k=p.store[0].data_ptr(), v=p.store[1].data_ptr(), k_meta=None, v_meta=None,
+                     page_table=at["tables"] + 4 * 4 * max_pages, format=fmt, n_kv_heads=nkv, head_dim=hd)
+    step = n_dec * nq * hd * 2
+    ok(dev.vv_attn_prefill(2, x[0].data_ptr() + step, C.addressof(one), out.data_ptr() + step, nq, chunk, 90, 90 + chunk,
+                           True, None, stream()))
+    torch.cuda.synchronize()
+    # 101, 64, 2 and 201 positions fit the pages that 100, 63, 1 and 200 have; 160 need one more than 90
+    assert d["counts"].tolist() == [n_free - 1, rows, 0] and d["lens"].tolist() == [101, 64, 2, 201, 160]
+    p.tables, p.lens = d["tables"].cpu().numpy(), d["lens"].tolist()
+    now = [p.values(i) for i in range(5)]
+    for i in range(5):                                                   # what was cached is untouched
+        assert all(np.array_equal(a, b[:len(a)]) for a, b in zip(held[i], now[i]))
+    q, got = (t.float().cpu().numpy().astype(np.float64) for t in (x[0], out))
+    for r in range(rows):
+        i = min(r, 4)
+        n = p.lens[i] if i < 4 else 90 + r - 4 + 1
+        k, v = (t[:n] for t in now[i])
+        want, mag = attend(q[r], k, v)
+        assert (np.abs(got[r] - want) <= attend_bound(want, mag, n, np.abs(v).max())).all(), f"row {r}"
