@@ -165,12 +165,12 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan(PlanArgs a) {
 // three flops a value: bound by memory, or by its latency when there are few rows.
 // A thread's item is one pair of chunks (c, c + hd/16) of one head: the eight rotary pairs (d, d + hd/2), or for V just
 // sixteen values. Heads are counted q, then k, then v. A workgroup owns whole rows, one where a row has 128 items or
-// more: its threads ask for their items first, then compute the rows' cosines and sines, one pair a thread, into LDS
+// more: its threads ask for their items first, then compute the row's cosines and sines, one pair a thread, into LDS
 // under the loads, and rotate and store behind one barrier. Launches of 2 MiB and more store non-temporally (14449
-// rows: 47.3 us, 55 without) but load ordinarily: q, k and v were just written by the projections, and what of them is
-// still cached is worth more than the hint (4096 rows: 12.7 us, 15.2 with it; 14449 rows 47.3 and 46.7). Measured at
-// 28 + 4 heads of 128 with biases: 16 rows 4.0 us, 2161 rows into an E4M3 pool 8.9, 4096 rows 12.7 (6.0 TB/s), 14449 rows
-// 47.3 us (5.6 TB/s; 44.3 without biases).
+// rows: 45.8 us, 50.5 without) but load ordinarily: q, k and v were just written by the projections, and what of them is
+// still cached is worth more than the hint (4096 rows: 12.5 us, 14.9 with it; 14449 rows 45.8 and 45.1). Measured at
+// 28 + 4 heads of 128 with biases: 16 rows 3.9 us, 2161 rows into an E4M3 pool 8.6, 4096 rows 12.5 (6.0 TB/s), 14449 rows
+// 45.8 us (5.8 TB/s), into an E4M3 pool 45.6.
 struct AppendArgs {
     const h16* q;
     const h16* k;
@@ -225,81 +225,133 @@ __device__ __forceinline__ void store_values(void* store, size_t at, const Chunk
 constexpr int kAppendThreads = 1024;      // at most
 constexpr int kAppendRows = 8;            // rows a workgroup owns, at most
 
-template <int kHd, int kFmt, bool kStream, bool kOneRow>
+// (These take the arguments by value: behind a reference, a choice between two of them becomes a choice between two
+// addresses, and the compiler keeps the struct in scratch memory - 181 us instead of 46 at 14449 rows.)
+// What a thread does with its item once everything has arrived: bias, rotation, one rounding, the stores.
+template <int kHd, int kFmt, bool kStream>
+__device__ __forceinline__ void finish_item(AppendArgs a, size_t row, int64_t slot, int kind, int h, int c,
+                                            const Chunk& lo, const Chunk& hi, bool biased, const Chunk& b0,
+                                            const Chunk& b1, const float* cosines, const float* sines, bool live) {
+    constexpr int kItems = kHd / 16, kHalf = kHd / 2;
+    f32x8 x0 = unpack(lo), x1 = unpack(hi);
+    if (biased) {
+        const f32x8 y0 = unpack(b0), y1 = unpack(b1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x0[i] += y0[i];
+            x1[i] += y1[i];
+        }
+    }
+    if (kind != 2) {
+        const f32x8 cv = *reinterpret_cast<const f32x8*>(cosines + 8 * c);
+        const f32x8 sv = *reinterpret_cast<const f32x8*>(sines + 8 * c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const Pair y = rotate(x0[i], x1[i], cv[i], sv[i]);
+            x0[i] = y.lo;
+            x1[i] = y.hi;
+        }
+    }
+    if (!live || slot < 0 || slot >= a.n_slots) return;
+    const Chunk y0 = pack(x0), y1 = pack(x1);
+    if (kind == 0) {
+        Chunk* dst = reinterpret_cast<Chunk*>(a.q_out + (row * a.nq + h) * kHd) + c;
+        store_chunk_as<kStream>(dst, y0);
+        store_chunk_as<kStream>(dst + kItems, y1);
+    } else {
+        void* store = kind == 1 ? a.k_store : a.v_store;
+        const size_t at = ((size_t)slot * a.nkv + h) * kHd + 8 * c;
+        store_values<kFmt, kStream>(store, at, y0);
+        store_values<kFmt, kStream>(store, at + kHalf, y1);
+    }
+}
+// Head `head` of a row, counted q, k, v: which tensor, and the head in it.
+__device__ __forceinline__ int kind_of(AppendArgs a, int head, int& h) {
+    const int kind = head < a.nq ? 0 : head < a.nq + a.nkv ? 1 : 2;
+    h = kind == 0 ? head : kind == 1 ? head - a.nq : head - a.nq - a.nkv;
+    return kind;
+}
+template <int kHd>
+__device__ __forceinline__ const Chunk* item_of(AppendArgs a, size_t row, int kind, int h, int c) {
+    return reinterpret_cast<const Chunk*>((kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
+                                          (row * (kind == 0 ? a.nq : a.nkv) + h) * kHd) + c;
+}
+template <int kHd>
+__device__ __forceinline__ const Chunk* bias_of(AppendArgs a, int kind, int h, int c) {      // or nullptr
+    const h16* bias = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
+    return bias ? reinterpret_cast<const Chunk*>(bias + (size_t)h * kHd) + c : nullptr;
+}
+
+// One row a workgroup, one item a thread (rows of 128 to 1024 items). Position and slot are asked for before the tensors:
+// memory returns in order, so the angles are computed while the tensors fly. They go through the vector path, for
+// which a zero that the compiler cannot see through stands in: as the scalar loads it makes of a workgroup's one slot
+// and position, 14449 rows take 46.5 us instead of 45.8. (Two rows a workgroup: 45.7 us, and 9.2 instead of 8.6 for 2161 rows into an
+// E4M3 pool; three rows are slower throughout.)
+template <int kHd, int kFmt, bool kStream>
+__global__ __launch_bounds__(kAppendThreads) void append_row(AppendArgs a, FreqTable freqs) {
+    constexpr int kItems = kHd / 16, kHalf = kHd / 2;
+    __shared__ __attribute__((aligned(16))) float cs_cos[kHalf], cs_sin[kHalf];
+    const int tid = (int)threadIdx.x;
+    const size_t row = blockIdx.x;
+    const int per_row = (a.nq + 2 * a.nkv) * kItems, item = min(tid, per_row - 1);
+    int zero = 0;
+    asm volatile("" : "+v"(zero));
+    int my_pos = a.positions[row + zero];
+    float my_freq = freqs.f[tid % kHalf];
+    const int64_t slot = a.slots[row + zero];
+    const int c = item % kItems;
+    int h;
+    const int kind = kind_of(a, item / kItems, h);
+    const Chunk* p = item_of<kHd>(a, row, kind, h, c);
+    const Chunk lo = load_chunk(p), hi = load_chunk(p + kItems);
+    const Chunk* bp = bias_of<kHd>(a, kind, h, c);
+    Chunk b0 = {}, b1 = {};
+    if (bp) {
+        b0 = load_chunk(bp);
+        b1 = load_chunk(bp + kItems);
+    }
+    asm volatile("" : "+v"(my_pos), "+v"(my_freq));
+    if (tid < kHalf) {
+        float s, cc;
+        sincosf((float)my_pos * my_freq, &s, &cc);
+        cs_cos[tid] = cc;
+        cs_sin[tid] = s;
+    }
+    __syncthreads();
+    finish_item<kHd, kFmt, kStream>(a, row, slot, kind, h, c, lo, hi, bp != nullptr, b0, b1, cs_cos, cs_sin, tid < per_row);
+}
+
+// Several rows a workgroup where they are short, several rounds of items where they are very long.
+template <int kHd, int kFmt>
 __global__ __launch_bounds__(kAppendThreads) void append_rows(AppendArgs a, FreqTable freqs, int rows_per_wg) {
     constexpr int kItems = kHd / 16, kHalf = kHd / 2;
     __shared__ __attribute__((aligned(16))) float cs_cos[kAppendRows * kHalf], cs_sin[kAppendRows * kHalf];
     const int tid = (int)threadIdx.x;
-    const int row0 = (int)blockIdx.x * (kOneRow ? 1 : rows_per_wg), rows = kOneRow ? 1 : min(rows_per_wg, a.rows - row0);
+    const int row0 = (int)blockIdx.x * rows_per_wg, rows = min(rows_per_wg, a.rows - row0);
     const int per_row = (a.nq + 2 * a.nkv) * kItems, items = rows * per_row;
-    // Asked for before the tensors: memory returns in order, so the angles are computed while the tensors fly. Through the
-    // vector path, for which a zero that the compiler cannot see through stands in: as scalar loads, which it makes of a
-    // workgroup's one slot and position, 14449 rows of 28 + 4 heads take 51 us instead of 47.
-    int zero = 0;
-    asm volatile("" : "+v"(zero));
-    int my_pos = a.positions[row0 + min(tid / kHalf, rows - 1) + zero];
-    float my_freq = freqs.f[tid % kHalf];
-    for (int base = 0; base < items; base += (int)blockDim.x) {       // one round unless a row has more than 1024 items
-        const int item = min(base + tid, items - 1);
-        const int r = kOneRow ? 0 : item / per_row, in_row = item - r * per_row;
-        const int head = in_row / kItems, c = in_row % kItems;
-        const int kind = head < a.nq ? 0 : head < a.nq + a.nkv ? 1 : 2;
-        const int h = kind == 0 ? head : kind == 1 ? head - a.nq : head - a.nq - a.nkv;
+    for (int i = tid; i < rows * kHalf; i += (int)blockDim.x) {
+        float s, cc;
+        sincosf((float)a.positions[row0 + i / kHalf] * freqs.f[i % kHalf], &s, &cc);
+        cs_cos[i] = cc;
+        cs_sin[i] = s;
+    }
+    __syncthreads();
+    for (int item = tid; item < items; item += (int)blockDim.x) {
+        const int r = item / per_row, in_row = item - r * per_row, c = in_row % kItems;
         const size_t row = (size_t)(row0 + r);
-        const h16* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + (row * (kind == 0 ? a.nq : a.nkv) + h) * kHd;
-        const h16* bias = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
-        const Chunk* p = reinterpret_cast<const Chunk*>(src) + c;
-        const int64_t slot = a.slots[row + zero];
+        int h;
+        const int kind = kind_of(a, in_row / kItems, h);
+        const int64_t slot = a.slots[row];
+        const Chunk* p = item_of<kHd>(a, row, kind, h, c);
         const Chunk lo = load_chunk(p), hi = load_chunk(p + kItems);
+        const Chunk* bp = bias_of<kHd>(a, kind, h, c);
         Chunk b0 = {}, b1 = {};
-        if (bias) {
-            const Chunk* bp = reinterpret_cast<const Chunk*>(bias + (size_t)h * kHd) + c;
+        if (bp) {
             b0 = load_chunk(bp);
             b1 = load_chunk(bp + kItems);
         }
-        if (base == 0) {
-            asm volatile("" : "+v"(my_pos), "+v"(my_freq));
-            for (int i = tid; i < rows * kHalf; i += (int)blockDim.x) {
-                float s, cc;
-                const bool mine = i == tid;
-                sincosf((float)(mine ? my_pos : a.positions[row0 + i / kHalf]) * (mine ? my_freq : freqs.f[i % kHalf]),
-                        &s, &cc);
-                cs_cos[i] = cc;
-                cs_sin[i] = s;
-            }
-            __syncthreads();
-        }
-        f32x8 x0 = unpack(lo), x1 = unpack(hi);
-        if (bias) {
-            const f32x8 y0 = unpack(b0), y1 = unpack(b1);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x0[i] += y0[i];
-                x1[i] += y1[i];
-            }
-        }
-        if (kind != 2) {
-            const f32x8 cv = *reinterpret_cast<const f32x8*>(&cs_cos[r * kHalf + 8 * c]);
-            const f32x8 sv = *reinterpret_cast<const f32x8*>(&cs_sin[r * kHalf + 8 * c]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const Pair y = rotate(x0[i], x1[i], cv[i], sv[i]);
-                x0[i] = y.lo;
-                x1[i] = y.hi;
-            }
-        }
-        if (base + tid >= items || slot < 0 || slot >= a.n_slots) continue;
-        const Chunk y0 = pack(x0), y1 = pack(x1);
-        if (kind == 0) {
-            Chunk* dst = reinterpret_cast<Chunk*>(a.q_out + (row * a.nq + h) * kHd) + c;
-            store_chunk_as<kStream>(dst, y0);
-            store_chunk_as<kStream>(dst + kItems, y1);
-        } else {
-            void* store = kind == 1 ? a.k_store : a.v_store;
-            const size_t at = ((size_t)slot * a.nkv + h) * kHd + 8 * c;
-            store_values<kFmt, kStream>(store, at, y0);
-            store_values<kFmt, kStream>(store, at + kHalf, y1);
-        }
+        finish_item<kHd, kFmt, false>(a, row, slot, kind, h, c, lo, hi, bp != nullptr, b0, b1, cs_cos + r * kHalf,
+                                      cs_sin + r * kHalf, true);
     }
 }
 
@@ -401,6 +453,7 @@ vv_status_t vv_rope_kv_append_dev(const void* q, const void* k, const void* v, c
     if (fp8 && !chunks) return VV_ERR_UNSUPPORTED;
     if (chunks && (head_dim == 128 || head_dim == 64)) {
         const int64_t per_row = (int64_t)(n_q_heads + 2 * n_kv_heads) * (head_dim / 16);
+        const bool one = per_row >= 128 && per_row <= vv::kAppendThreads;
         int rows = per_row >= 128 ? 1 : (int)(256 / per_row);
         if (rows > vv::kAppendRows) rows = vv::kAppendRows;
         if (rows > n_rows) rows = n_rows;
@@ -408,11 +461,11 @@ vv_status_t vv_rope_kv_append_dev(const void* q, const void* k, const void* v, c
         const unsigned threads = (unsigned)(want < vv::kAppendThreads ? want : vv::kAppendThreads);
         const dim3 grid((unsigned)((n_rows - 1) / rows + 1));
         const bool stream = vv::use_streaming(2u * (size_t)n_rows * (size_t)per_row * 32u);
-#define VV_APPEND(H, F)                                                                                \
-    do {                                                                                               \
-        if (rows > 1)    vv::append_rows<H, vv::F, false, false><<<grid, threads, 0, st>>>(a, freqs, rows); \
-        else if (stream) vv::append_rows<H, vv::F, true, true><<<grid, threads, 0, st>>>(a, freqs, rows);   \
-        else             vv::append_rows<H, vv::F, false, true><<<grid, threads, 0, st>>>(a, freqs, rows);  \
+#define VV_APPEND(H, F)                                                                        \
+    do {                                                                                       \
+        if (one && stream) vv::append_row<H, vv::F, true><<<grid, threads, 0, st>>>(a, freqs); \
+        else if (one)      vv::append_row<H, vv::F, false><<<grid, threads, 0, st>>>(a, freqs); \
+        else               vv::append_rows<H, vv::F><<<grid, threads, 0, st>>>(a, freqs, rows); \
     } while (0)
         if (head_dim == 64)                       VV_APPEND(64, kFmtFp16);
         else if (!fp8)                            VV_APPEND(128, kFmtFp16);
