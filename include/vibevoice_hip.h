@@ -667,7 +667,8 @@ vv_status_t vv_kv_page_map_dev(int* page_table, int first, int n, const int* pag
  * free_pages is not written: a finished sequence's pages return by being written from free_pages[*n_free] on.
  * lens_out may be cache_lens and n_free_out may be n_free (a captured step that advances itself); one workgroup then
  * fills all rows. Other overlaps are the caller's mistake; lens_out == new_lens and counts == n_free or n_free_out are
- * refused with VV_ERR_INVALID_ARG, max_rows above 2^30 with VV_ERR_UNSUPPORTED. Takes the place of vv_kv_page_map_dev and of the host's slot arithmetic per sequence. */
+ * refused with VV_ERR_INVALID_ARG; more than 2^30 rows or sequences, or tables of more than 2^31 - 1 positions, with
+ * VV_ERR_UNSUPPORTED. Takes the place of vv_kv_page_map_dev and of the host's slot arithmetic per sequence. */
 vv_status_t vv_kv_page_plan_dev(const int* new_lens, const int* cache_lens, int n_seqs, int* page_tables,
                                 int max_pages, const int* free_pages, const int* n_free, int* lens_out,
                                 int* row_starts, int* positions, int64_t* slots, int max_rows, int* n_free_out,
@@ -683,7 +684,8 @@ vv_status_t vv_kv_page_plan_dev(const int* new_lens, const int* cache_lens, int 
  * included. Slots must differ from one another; of two rows with one slot either may win, vector piece by piece.
  * kv_format FP16: any even head_dim <= 256 and 2-byte alignment (head_dim 64 and 128 with everything 16-byte aligned
  * take the vector kernel); FP8 E4M3 / E5M2: head_dim 128, 16-byte aligned tensors, 8-byte aligned stores. Other
- * formats, shapes and alignments: VV_ERR_UNSUPPORTED. */
+ * formats, shapes and alignments, and more rows than a launch of 2^32 threads holds (16 to 1024 threads a row), are
+ * VV_ERR_UNSUPPORTED. */
 vv_status_t vv_rope_kv_append_dev(const void* q, const void* k, const void* v, const void* q_bias,
                                   const void* k_bias, const void* v_bias, const int* positions,
                                   const int64_t* slots, void* q_out, void* k_store, void* v_store, int n_rows,

@@ -129,3 +129,12 @@ def test_the_plain_plan_hands_out_pages_like_a_stack():
     assert got["counts"].tolist() == [-2, 131, 2]        # 2 less the 1 + 2 + 1 asked for up to the last one served
     assert (got["slots"][1:130] == -1).all() and got["slots"][130] == 7 * PAGE + 3
     assert pages_of(0) == 0 and pages_of(1) == 1 and pages_of(64) == 1 and pages_of(65) == 2
+
+
+def test_counts_past_what_a_launch_or_32_bits_hold_are_refused():
+    assert plan_call(n_seqs=(1 << 30) + 1) == dev.VV_ERR_UNSUPPORTED
+    assert plan_call(max_pages=1 << 25) == dev.VV_ERR_UNSUPPORTED                # 2^31 positions
+    # rows of 28 + 2 * 4 heads of 8 items run 320 threads: floor((2^32 - 1) / 320) of them fit a launch
+    wide = dict(n_q_heads=28, n_kv_heads=4)
+    assert append_call(n_rows=(2**32 - 1) // 320 + 1, **wide) == dev.VV_ERR_UNSUPPORTED
+    assert append_call(n_rows=(2**32 - 1) // 256 + 1, head_dim=126) == dev.VV_ERR_UNSUPPORTED

@@ -169,7 +169,7 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan(PlanArgs a) {
 // under the loads, and rotate and store behind one barrier. Launches of 2 MiB and more store non-temporally (14449
 // rows: 45.8 us, 50.5 without) but load ordinarily: q, k and v were just written by the projections, and what of them is
 // still cached is worth more than the hint (4096 rows: 12.5 us, 14.9 with it; 14449 rows 45.8 and 45.1). Measured at
-// 28 + 4 heads of 128 with biases: 16 rows 3.9 us, 2161 rows into an E4M3 pool 8.6, 4096 rows 12.5 (6.0 TB/s), 14449 rows
+// 28 + 4 heads of 128 with biases: 16 rows 2.9 us, 2161 rows into an E4M3 pool 8.6, 4096 rows 12.5 (6.0 TB/s), 14449 rows
 // 45.8 us (5.8 TB/s), into an E4M3 pool 45.6.
 struct AppendArgs {
     const h16* q;
@@ -412,7 +412,8 @@ vv_status_t vv_kv_page_plan_dev(const int* new_lens, const int* cache_lens, int 
     if (!new_lens || !cache_lens || !page_tables || !free_pages || !n_free || !lens_out || !row_starts || !counts)
         return VV_ERR_NULL_PTR;
     if (max_pages <= 0 || max_rows < 0) return VV_ERR_INVALID_ARG;
-    if (max_rows > (1 << 30)) return VV_ERR_UNSUPPORTED;           // a saturated row count is past every row then
+    // A saturated row count is past every row then; the loop over sequences, and a position, stay within 32 bits.
+    if (max_rows > (1 << 30) || n_seqs > (1 << 30) || (int64_t)max_pages * vv::kPage > INT32_MAX) return VV_ERR_UNSUPPORTED;
     if (max_rows > 0 && (!positions || !slots)) return VV_ERR_NULL_PTR;
     if (lens_out == new_lens || counts == n_free || counts == n_free_out) return VV_ERR_INVALID_ARG;
     vv::PlanArgs a = {new_lens, cache_lens, page_tables, free_pages, n_free, lens_out, row_starts, positions, slots,
@@ -451,6 +452,8 @@ vv_status_t vv_rope_kv_append_dev(const void* q, const void* k, const void* v, c
                         (fp8 ? vv::aligned8(k_store) && vv::aligned8(v_store)
                              : vv::aligned16(k_store) && vv::aligned16(v_store));
     if (fp8 && !chunks) return VV_ERR_UNSUPPORTED;
+    // A launch holds less than 2^32 threads.
+    auto too_many = [](size_t wgs, size_t threads) { return wgs > UINT32_MAX / threads; };
     if (chunks && (head_dim == 128 || head_dim == 64)) {
         const int64_t per_row = (int64_t)(n_q_heads + 2 * n_kv_heads) * (head_dim / 16);
         const bool one = per_row >= 128 && per_row <= vv::kAppendThreads;
@@ -460,6 +463,7 @@ vv_status_t vv_rope_kv_append_dev(const void* q, const void* k, const void* v, c
         const int64_t want = (rows * per_row + vv::kWave - 1) / vv::kWave * vv::kWave;
         const unsigned threads = (unsigned)(want < vv::kAppendThreads ? want : vv::kAppendThreads);
         const dim3 grid((unsigned)((n_rows - 1) / rows + 1));
+        if (too_many(grid.x, threads)) return VV_ERR_UNSUPPORTED;
         const bool stream = vv::use_streaming(2u * (size_t)n_rows * (size_t)per_row * 32u);
 #define VV_APPEND(H, F)                                                                        \
     do {                                                                                       \
@@ -473,6 +477,7 @@ vv_status_t vv_rope_kv_append_dev(const void* q, const void* k, const void* v, c
         else                                      VV_APPEND(128, kFmtE5M2);
 #undef VV_APPEND
     } else {
+        if (too_many((size_t)n_rows, vv::kBlock)) return VV_ERR_UNSUPPORTED;
         vv::append_generic<<<dim3((unsigned)n_rows), vv::kBlock, 0, st>>>(a, freqs);
     }
     return vv::launch_status();
