@@ -65,6 +65,15 @@ struct BatchArgs {
     float scale_log2;
 };
 
+// A score's product with the softmax's scale, rounded by itself. Fused into the subtraction of the maximum (which was
+// rounded), the largest score's exponent would be off by half a step of the score: 8 at 2^27, which FP16 inputs reach
+// (65504^2 sqrt(128) log2(e) is 2^36), and the probability past what FP16 holds. Rounded first, the largest score is its
+// maximum to the bit.
+__device__ __forceinline__ float scaled(float score, float scale) {
+#pragma clang fp contract(off)
+    return score * scale;
+}
+
 __device__ __forceinline__ int seen_len(const BatchArgs& a, int s) { return min(max(a.lens[s], 0), a.max_pages * kPage); }
 __device__ __forceinline__ int pages_of(int len) { return (len + kPage - 1) / kPage; }
 
@@ -365,12 +374,14 @@ __global__ __launch_bounds__(kBatchThreads, 2) void decode_batch(BatchArgs a) {
                             }
                         }
                     }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sc[r] = scaled(sc[r], a.scale_log2);
                     if (in_use < 16) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) sc[r] = position(4 * j + r) < in_use ? sc[r] : -INFINITY;
                     }
                     float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-                    mx = max_xor32(max_xor16(mx)) * a.scale_log2;
+                    mx = max_xor32(max_xor16(mx));
                     const float m_new = fmaxf(m, mx);
                     const float m_use = m_new == -INFINITY ? 0.0f : m_new;
                     if (__builtin_amdgcn_ballot_w64(m_new > m) != 0) {
@@ -385,7 +396,7 @@ __global__ __launch_bounds__(kBatchThreads, 2) void decode_batch(BatchArgs a) {
                     h16x4 pf;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float pr = exp2_fast(fmaf(sc[r], a.scale_log2, kLift - m_use));
+                        const float pr = exp2_fast(sc[r] - m_use + kLift);
                         l += pr;
                         pf[r] = (h16)pr;
                     }
@@ -572,7 +583,7 @@ __global__ __launch_bounds__(kWave) void decode_batch_generic(BatchArgs a, int h
             dot = d < head_dim ? fmaf(qv[i], (float)k[d], dot) : dot;
             vv4[i] = d < head_dim ? (float)v[d] : 0.0f;
         }
-        const float s = wave_sum(dot) * a.scale_log2;
+        const float s = scaled(wave_sum(dot), a.scale_log2);
         const float m_new = fmaxf(m, s), m_use = m_new == -INFINITY ? 0.0f : m_new;
         const float alpha = exp2_fast(m - m_use), p = exp2_fast(s - m_use);
         m = m_new;
