@@ -1,0 +1,44 @@
+"""CPU checks of what the batched-serving tests rest on: the bounds that attention is held to reject an answer that lost a
+page, a tail or a single position."""
+import numpy as np
+import pytest
+
+from batch_util import (PAGE, attend, attend_bound_lifted, census, census_bound, pages_of, slots_of)
+
+
+def draw(n, nq, nkv, hd, rng, sharp=2.0):
+    """Inputs of the distribution that the GPU tests' pools have."""
+    q = rng.normal(size=(nq, hd)) * sharp * 2 * hd ** -0.25
+    k = rng.normal(size=(n, nkv, hd)) * 2 * hd ** -0.25
+    return tuple(x.astype(np.float16).astype(np.float64) for x in (q, k, rng.normal(size=(n, nkv, hd))))
+
+
+def worst(got, ref, mag, n, v):
+    return (np.abs(got - ref) / attend_bound_lifted(ref, mag, n, np.abs(v).max())).max()
+
+
+@pytest.mark.parametrize("n", [1000, 14449, 20000])
+def test_the_bound_sees_a_lost_page_and_a_lost_tail(n):
+    rng = np.random.default_rng(n)
+    q, k, v = draw(n, 4, 2, 128, rng)
+    ref, mag = attend(q, k, v)
+    for page in rng.integers(0, n // PAGE, 4):
+        drop = np.arange(page * PAGE, (page + 1) * PAGE)
+        assert worst(attend(q, np.delete(k, drop, 0), np.delete(v, drop, 0))[0], ref, mag, n, v) > 1.0
+    assert worst(attend(q, k[:-17], v[:-17])[0], ref, mag, n, v) > 1.0
+    assert worst(ref.astype(np.float16).astype(np.float64), ref, mag, n, v) <= 1.0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,lost", [(65, 1), (14449, 1), (20000, 1), (1 << 20, PAGE)])
+def test_the_census_sees_what_is_lost_or_counted_twice(n, lost, hd):
+    rng = np.random.default_rng(n)
+    pages = rng.integers(0, 300, pages_of(n))
+    want = census(pages, n, hd)
+    at = slots_of(pages.astype(np.int32), n) // PAGE % hd
+    assert np.array_equal(want, np.bincount(at, minlength=hd) / n)
+    for begin in rng.integers(0, n // lost, 4) * lost:
+        some = at[begin:begin + lost]
+        for wrong in (np.bincount(np.delete(at, np.arange(begin, begin + lost)), minlength=hd) / (n - lost),
+                      np.bincount(np.append(at, some), minlength=hd) / (n + lost)):
+            assert (np.abs(wrong - want) > census_bound(want)).any()
