@@ -647,7 +647,16 @@ vv_status_t vv_kv_page_map_dev(int* page_table, int first, int n, const int* pag
 /* A pool is one layer's K and V stores [n_pages * 64][n_kv_heads][head_dim] as vv_kv_view_t describes them; page p
  * holds rows 64 p .. 64 p + 63. Each of n_seqs sequences has a row of max_pages page ids (int32) in page_tables and
  * its length in cache_lens: position t of sequence i lies in row ("slot")
- * page_tables[i * max_pages + t / 64] * 64 + t % 64. Sequences may share pages that none of them writes. */
+ * page_tables[i * max_pages + t / 64] * 64 + t % 64. Sequences may share pages that none of them writes.
+ *
+ * Rows and sequences: vv_kv_page_plan_dev packs rows by the running sum of new_lens, vv_attn_decode_batch takes row i of
+ * q and out for sequence i. The two agree where every sequence before the last one decoded asks for exactly one row. So in
+ * a pool of slots that is served by one captured step each slot asks for one row (new_lens all 1, max_rows >= n_seqs)
+ * whether it decodes or not, and one that has nothing to decode says so by a negative length: -1 where it holds nothing,
+ * -1 - len where it waits with len positions (the length goes back to len when it goes on). It is refused, so it takes
+ * no page, keeps its length and gets slot -1; its row is skipped by vv_rope_kv_append_dev and answered with zeros by
+ * vv_attn_decode_batch. new_lens[i] = 0 for it instead would give it no row, and every later sequence another one's
+ * query. */
 
 /* addition: the pages and slots of a step's new positions, from the lengths, all on the device: sequence i holds
  * cache_lens[i] positions and gets new_lens[i] more (<= 0: none), in ceil((len + new) / 64) - ceil(len / 64) new
@@ -655,7 +664,8 @@ vv_status_t vv_kv_page_map_dev(int* page_table, int first, int n, const int* pag
  * order and through each one's positions, is free_pages[*n_free - 1 - j]; its id goes into the sequence's table.
  * A sequence is refused, gets nothing and keeps its length when its positions would not fit max_pages pages, when its
  * rows would end past max_rows, when its length is negative, or when it needs pages and the running sum of needed
- * pages (in order, those refused for want of pages counted: none overtakes) passes *n_free.
+ * pages (in order, those refused for want of pages counted: none overtakes) passes *n_free. Its rows have slot -1:
+ * nothing is appended for them, and what attention then answers for it is of no use to the caller.
  *   lens_out[n_seqs]       lengths after the step
  *   row_starts[n_seqs + 1] first packed row of each sequence: the running sum of new_lens (refused ones included, so
  *                          rows keep the places the caller packed them in), held at max_rows
@@ -696,12 +706,12 @@ vv_status_t vv_rope_kv_append_dev(const void* q, const void* k, const void* v, c
  * below one and for head counts that do not divide. */
 size_t vv_attn_decode_batch_scratch_bytes(int n_seqs, int n_q_heads, int n_kv_heads, int head_dim);
 /* addition: vv_attn_decode for n_seqs sequences at once: out[i] = attention of the one query row q[i]
- * [n_q_heads][head_dim] against the first cache_lens[i] positions behind row i of kv->page_table ([n_seqs][max_pages],
+ * [n_q_heads][head_dim] (row i for sequence i: q and out hold n_seqs rows, whatever a plan packed into them) against the first cache_lens[i] positions behind row i of kv->page_table ([n_seqs][max_pages],
  * required here); out may be q. Lengths are read on the device, may differ as they like and size nothing on the host: a captured
  * step replays at any lengths. The pages of all sequences and KV heads are dealt out evenly over the workgroups,
  * whatever sequence they belong to; a row that several workgroups share is folded in page order, so a result
  * does not depend on timing (its last bits depend on where the batch's pages were cut).
- * cache_lens[i] <= 0: zeros. A length past 64 * max_pages is taken as that. Positions behind a page id outside
+ * cache_lens[i] <= 0: zeros (a slot that stands by, see above). A length past 64 * max_pages is taken as that. Positions behind a page id outside
  * [0, n_pages) count as masked; what the pool holds past a length or there is never used, NaN included.
  * FP16 pools of head_dim 64 and 128 with q and the stores 16-byte aligned run on the matrix cores, any other
  * head_dim <= 256 or alignment on a slower kernel that needs no scratch; FP8 E4M3 / E5M2: head_dim 128, the same

@@ -1,9 +1,20 @@
 """CPU checks of what the batched-serving tests rest on: the bounds that attention is held to reject an answer that lost a
-page, a tail or a single position."""
+page, a tail or a single position, and a slot of a fixed pool that stands by keeps its row."""
 import numpy as np
 import pytest
 
-from batch_util import (PAGE, attend, attend_bound_lifted, census, census_bound, pages_of, slots_of)
+from batch_util import (PAGE, attend, attend_bound_lifted, census, census_bound, pages_of, plan, slots_of)
+
+
+def test_a_slot_that_stands_by_keeps_its_row():
+    """A negative length with one row asked for: refused, so it gets no page and keeps its length, but its row stays its
+    own; every other slot's row is its index."""
+    tables = np.array([[4, -1], [-1, -1], [5, -1], [6, -1]], np.int32)
+    got = plan([1, 1, 1, 1], [10, -1, -1 - 20, 63], tables, [1, 2], 2, 4)
+    assert got["row_starts"].tolist() == [0, 1, 2, 3, 4]
+    assert got["lens"].tolist() == [11, -1, -21, 64] and got["counts"].tolist() == [2, 4, 2]
+    assert got["slots"].tolist() == [4 * PAGE + 10, -1, -1, 6 * PAGE + 63]
+    assert np.array_equal(got["tables"], tables) and got["n_free"] == 2
 
 
 def draw(n, nq, nkv, hd, rng, sharp=2.0):
