@@ -40,6 +40,16 @@ def test_the_bound_sees_a_lost_page_and_a_lost_tail(n):
     assert worst(ref.astype(np.float16).astype(np.float64), ref, mag, n, v) <= 1.0
 
 
+@pytest.mark.parametrize("n", [4, 64, 190])
+def test_the_bound_sees_another_answer(n):
+    """Zeros, the other sign, the heads in reverse, uniform weights and another query's answer, at the lengths and of the
+    distribution that the serving loops have."""
+    q, k, v = draw(n, 8, 2, 128, np.random.default_rng(n))
+    ref, mag = attend(q, k, v)
+    for wrong in (np.zeros_like(ref), -ref, ref[::-1], np.repeat(v.mean(0), 4, 0), attend(q[::-1], k, v)[0]):
+        assert worst(wrong, ref, mag, n, v) > 1.0
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("n,lost", [(65, 1), (14449, 1), (20000, 1), (1 << 20, PAGE)])
 def test_the_census_sees_what_is_lost_or_counted_twice(n, lost, hd):

@@ -190,3 +190,30 @@ def test_slots_decode_stand_by_and_are_refused(fmt, captured):
     assert refused > 0 and waited == 6 and (s.lens > 0).sum() == 6
     if captured:
         dev.vv_dev_graph_destroy(graph)
+
+
+@pytest.mark.parametrize("fmt", [FP16, E4M3, E5M2])
+@pytest.mark.parametrize("captured", [False, True])
+def test_every_slot_decodes(fmt, captured):
+    """All slots decode from the first step on, from prompts that end at and around a page's end; two fill their tables
+    and are refused from there on."""
+    prompts = np.array([3, 63, 64, 130, 1, 191])
+    n, rows = len(prompts), int(prompts.sum())
+    s = Slots(n, 3 * n, fmt, seed=50 + fmt)
+    s.lens[:] = 0
+    s.push()
+    big, st = s.rows(rows), torch.cuda.Stream()
+    s.step(big, rows, prompts, s.fill(big), lambda: s.launch(big, rows, st.cuda_stream, attention=False), attention=False)
+    small, graph = s.rows(n), C.c_void_p()
+    if captured:
+        torch.cuda.synchronize()
+        ok(dev.vv_dev_graph_begin(st.cuda_stream))
+        s.launch(small, n, st.cuda_stream)
+        ok(dev.vv_dev_graph_end(st.cuda_stream, C.byref(graph)))
+    for step in range(66):
+        x = s.fill(small)
+        s.step(small, n, np.ones(n, int), x, (lambda: ok(dev.vv_dev_graph_launch(graph, st.cuda_stream))) if captured
+               else (lambda: s.launch(small, n, st.cuda_stream)))
+    assert s.lens.tolist() == [69, 129, 130, 192, 67, 192]
+    if captured:
+        dev.vv_dev_graph_destroy(graph)
