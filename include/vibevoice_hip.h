@@ -715,10 +715,11 @@ size_t vv_attn_decode_batch_scratch_bytes(int n_seqs, int n_q_heads, int n_kv_he
  * [0, n_pages) count as masked; what the pool holds past a length or there is never used, NaN included.
  * FP16 pools of head_dim 64 and 128 with q and the stores 16-byte aligned run on the matrix cores, any other
  * head_dim <= 256 or alignment on a slower kernel that needs no scratch; FP8 E4M3 / E5M2: head_dim 128, the same
- * alignment. TurboQuant formats, more than 16384 query heads, 2^22 (sequence, KV head) pairs or 2^31 - 513
- * (sequence, KV head, page of the tables): VV_ERR_UNSUPPORTED. scratch: vv_attn_decode_batch_scratch_bytes() of device memory,
- * 16-byte aligned (smaller or unaligned: VV_ERR_INVALID_ARG); it needs no clearing, holds nothing between calls, and
- * calls that overlap need one each. */
+ * alignment, the codes read as torch.float8_e4m3fn and float8_e5m2 do: E4M3's 0x7F and 0xFF, which no store here writes,
+ * are NaN (vv_attn_decode and vv_kv_dequant_dev read them as 480 and -480). TurboQuant formats, more than 16384 query
+ * heads, 2^22 (sequence, KV head) pairs or 2^31 - 513 (sequence, KV head, page of the tables): VV_ERR_UNSUPPORTED.
+ * scratch: vv_attn_decode_batch_scratch_bytes() of device memory, 16-byte aligned (smaller or unaligned:
+ * VV_ERR_INVALID_ARG); it needs no clearing, holds nothing between calls, and calls that overlap need one each. */
 vv_status_t vv_attn_decode_batch(int backend, const void* q, const vv_kv_view_t* kv, void* out, int n_q_heads,
                                  int n_seqs, const int* cache_lens, int max_pages, int n_pages, void* scratch,
                                  size_t scratch_bytes, void* stream);
