@@ -676,7 +676,7 @@ vv_status_t vv_kv_page_map_dev(int* page_table, int first, int n, const int* pag
  *                          zero by what was missing), rows in use (row_starts[n_seqs]), sequences refused
  * free_pages is not written: a finished sequence's pages return by being written from free_pages[*n_free] on.
  * lens_out may be cache_lens and n_free_out may be n_free (a captured step that advances itself); one workgroup then
- * fills all rows. Other overlaps are the caller's mistake; lens_out == new_lens and counts == n_free or n_free_out are
+ * fills all rows (193 sequences with 2048 rows 13 us instead of 6, 32068 rows 104 instead of 5). Other overlaps are the caller's mistake; lens_out == new_lens and counts == n_free or n_free_out are
  * refused with VV_ERR_INVALID_ARG; more than 2^30 rows or sequences, or tables of more than 2^31 - 1 positions, with
  * VV_ERR_UNSUPPORTED. Takes the place of vv_kv_page_map_dev and of the host's slot arithmetic per sequence. */
 vv_status_t vv_kv_page_plan_dev(const int* new_lens, const int* cache_lens, int n_seqs, int* page_tables,
@@ -707,8 +707,8 @@ vv_status_t vv_rope_kv_append_dev(const void* q, const void* k, const void* v, c
 size_t vv_attn_decode_batch_scratch_bytes(int n_seqs, int n_q_heads, int n_kv_heads, int head_dim);
 /* addition: vv_attn_decode for n_seqs sequences at once: out[i] = attention of the one query row q[i]
  * [n_q_heads][head_dim] (row i for sequence i: q and out hold n_seqs rows, whatever a plan packed into them) against the first cache_lens[i] positions behind row i of kv->page_table ([n_seqs][max_pages],
- * required here); out may be q. Lengths are read on the device, may differ as they like and size nothing on the host: a captured
- * step replays at any lengths. The pages of all sequences and KV heads are dealt out evenly over the workgroups,
+ * required here); out may be q. Lengths are read on the device, may differ as they like and size nothing on the host:
+ * a captured step replays at any lengths. The pages of all sequences and KV heads are dealt out evenly over the workgroups,
  * whatever sequence they belong to; a row that several workgroups share is folded in page order, so a result
  * does not depend on timing (its last bits depend on where the batch's pages were cut).
  * cache_lens[i] <= 0: zeros (a slot that stands by, see above). A length past 64 * max_pages is taken as that. Positions behind a page id outside

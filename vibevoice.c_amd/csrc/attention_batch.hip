@@ -26,10 +26,12 @@
 //   join     Where a run ends a row (sequence, KV head) the four waves' states meet in LDS. A row that lies
 //            wholly inside a worker is finished there; otherwise each worker leaves (sum of p V, maximum, sum of p) in
 //            `parts`, and a second launch folds them in the order of their pages.
-// Measured at 28 + 4 heads of 128 (both launches, cache cold, three caches in turn): 1 x 14449 positions 14.4 us,
-// 8 x 2048 13.6, 24 of 0 .. 14449 64.6 us (5.5 TB/s), 32 of 12345 .. 14449 146.5 us (6.0 TB/s, 94 % of what a plain
-// read of 256-byte vectors reaches); 64 of 6001 .. 8192 in E4M3 84.6 us (5.5 TB/s). What is left below 100 MB is latency: 3.2
-// us until a worker's first loads go out (lengths, page ids), 3 until they are back, and 4.4 for the second launch.
+// Measured at 28 + 4 heads of 128 (both launches, from events around passes over three caches in turn): 1 x 14449
+// positions 14.7 us, 8 x 2048 13.8, 24 of 0 .. 14449 65 us (5.5 TB/s), 32 of 12345 .. 14449 147.3 us (5.9 TB/s, 93 % of
+// what a plain read of 256-byte vectors reaches; the first launch alone 144 us, 6.1); 64 of 6001 .. 8192 in E4M3 85.4 us
+// (5.5 TB/s). What is left below 100 MB is latency: 3.2 us until a worker's first loads go out (its arguments, the lengths -
+// of which a thread asks for four one after another, each awaited, from four sequences on -, the page ids), 3 until they
+// are back, and 4.4 for the second launch.
 #include <algorithm>
 
 #include "attn_common.hpp"
@@ -616,12 +618,12 @@ void launch_merge_of(const BatchArgs& a, int slices, hipStream_t st) {
 // The fewer rows, the more parts a row can have, and the more threads are put to one; but a workgroup costs its launch
 // also where a row has nothing to fold, which is what many rows mostly have. Measured (both launches) at 28 + 4 heads with
 // one head of 1024 threads / one of 256 / two of 256 / four of 256 / eight of 256 a workgroup, in us:
-//   one sequence of 14449 positions (4 rows)             14.5 / 16.0 / 19.7 / 27.7 / 43.4
-//   8 of 2048 (32 rows)                                  14.4 / 13.6 / 13.5 / 14.3 / 15.6
-//   one of 14449 and 39 of 60 (160 rows)                  -   / 17.7 / 20.5 / 25.9 / 35.9
-//   128 of 50 .. 150 (512 rows)                           -   / 14.5 / 14.5 / 14.4 / 14.0
-//   one of 32000 and 249 of 60 (1000 rows)                -   / 30.7 / 32.3 / 35.8 / 43.3
-//   1000 of 64 (4000 rows)                                -   / 39.7 / 37.2 / 35.7 / 34.9
+//   one sequence of 14449 positions (4 rows)             14.8 / 16.3 / 19.9 / 27.9 / 43.5
+//   8 of 2048 (32 rows)                                  14.6 / 13.8 / 13.8 / 14.5 / 15.8
+//   one of 14449 and 39 of 60 (160 rows)                 18.2 / 18.0 / 20.9 / 26.2 / 36.3
+//   128 of 50 .. 150 (512 rows)                          20.0 / 14.8 / 14.6 / 14.6 / 14.1
+//   one of 32000 and 249 of 60 (1000 rows)               34.7 / 31.1 / 32.6 / 36.1 / 43.8
+//   1000 of 64 (4000 rows)                               57.8 / 40.1 / 37.7 / 36.0 / 35.2
 template <int kHd>
 void launch_merge(const BatchArgs& a, int slices, hipStream_t st) {
     const int rows = a.n_seqs * a.n_kv_heads;
@@ -651,11 +653,13 @@ vv_status_t vv_attn_decode_batch(int backend, const void* q, const vv_kv_view_t*
     if (!kv->k || !kv->v || !kv->page_table) return VV_ERR_NULL_PTR;
     const bool fp8 = kv->format == vv::kFmtE4M3 || kv->format == vv::kFmtE5M2;
     if (kv->format != vv::kFmtFp16 && !(fp8 && kv->head_dim == 128)) return VV_ERR_UNSUPPORTED;
-    if (n_q_heads <= 0 || n_q_heads > (1 << 14) || kv->n_kv_heads <= 0 || n_q_heads % kv->n_kv_heads || kv->head_dim <= 0 || kv->head_dim > 256)
+    if (n_q_heads <= 0 || n_q_heads > (1 << 14) || kv->n_kv_heads <= 0 || n_q_heads % kv->n_kv_heads ||
+        kv->head_dim <= 0 || kv->head_dim > 256)
         return VV_ERR_UNSUPPORTED;
     if (max_pages <= 0 || n_pages <= 0) return VV_ERR_INVALID_ARG;
     // the list of (sequence, KV head, page) is counted in 32 bits, and a launch has a workgroup per row of it
-    if ((int64_t)n_seqs * kv->n_kv_heads > (1 << 22) || (int64_t)max_pages * vv::kPage > INT32_MAX || (int64_t)n_seqs * max_pages * kv->n_kv_heads > INT32_MAX - vv::kWorkers)
+    if ((int64_t)n_seqs * kv->n_kv_heads > (1 << 22) || (int64_t)max_pages * vv::kPage > INT32_MAX ||
+        (int64_t)n_seqs * max_pages * kv->n_kv_heads > INT32_MAX - vv::kWorkers)
         return VV_ERR_UNSUPPORTED;
     vv::BatchArgs a = {static_cast<const vv::h16*>(q), kv->k, kv->v, kv->page_table, cache_lens,
                        static_cast<vv::h16*>(out), nullptr, nullptr, n_q_heads, kv->n_kv_heads, n_seqs, max_pages,

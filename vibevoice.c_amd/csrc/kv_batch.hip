@@ -161,16 +161,19 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan(PlanArgs a) {
 // Row r: q_out[r] = rope(q[r] + bq), K[slot_r] = rope(k[r] + bk), V[slot_r] = v[r] + bv at position pos_r, in FP32 with
 // one rounding to FP16 (a biased value is not rounded before it is turned: separate calls, which store it there, are
 // off by sqrt(2) as much). The angle and the rotation are those of vv_rope_dev, and an FP8 code is that of the
-// FP16 value, so without biases the bits are those of vv_rope_qk_dev and vv_kv_store_dev on that row. A row moves 4 hd (nq + nkv) + 2 hd nkv (1 + bytes per stored value) bytes and does
-// three flops a value: bound by memory, or by its latency when there are few rows.
+// FP16 value, so without biases the bits are those of vv_rope_qk_dev and vv_kv_store_dev on that row. A row moves
+// 4 hd (nq + nkv) + 2 hd nkv b bytes, b the bytes of a stored value, and does three flops a value: bound by memory, or
+// by its latency when there are few rows.
 // A thread's item is one pair of chunks (c, c + hd/16) of one head: the eight rotary pairs (d, d + hd/2), or for V just
 // sixteen values. Heads are counted q, then k, then v. A workgroup owns whole rows, one where a row has 128 items or
 // more: its threads ask for their items first, then compute the row's cosines and sines, one pair a thread, into LDS
-// under the loads, and rotate and store behind one barrier. Launches of 2 MiB and more store non-temporally (14449
-// rows: 45.8 us, 50.5 without) but load ordinarily: q, k and v were just written by the projections, and what of them is
-// still cached is worth more than the hint (4096 rows: 12.5 us, 14.9 with it; 14449 rows 45.8 and 45.1). Measured at
-// 28 + 4 heads of 128 with biases: 16 rows 2.9 us, 2161 rows into an E4M3 pool 8.6, 4096 rows 12.5 (6.0 TB/s), 14449 rows
-// 45.8 us (5.8 TB/s), into an E4M3 pool 45.6.
+// under the loads, and rotate and store behind one barrier. The one-row kernel stores non-temporally in launches of 2 MiB
+// and more (14449 rows: 45.8 us, 50.5 without) but loads ordinarily: q, k and v were just written by the projections, and
+// what of them is still cached is worth more than the hint (4096 rows: 12.5 us, 14.9 with it; 14449 rows 45.8 and 45.1).
+// The kernel of short and of very long rows stores ordinarily at every size: at 14 + 2 heads of 64 with the hint, 1000 to
+// 4096 rows are the same, 14449 rows 14.4 us instead of 13.6, and only 60000 gain (55.9 instead of 60.4). Measured at 28 + 4
+// heads of 128 with biases: 16 rows 3.0 us, 2161 rows into an E4M3 pool 8.6, 4096 rows 12.5 (6.0 TB/s), 14449 rows
+// 46 us (5.8 TB/s), into an E4M3 pool 45.6.
 struct AppendArgs {
     const h16* q;
     const h16* k;
@@ -285,8 +288,8 @@ __device__ __forceinline__ const Chunk* bias_of(AppendArgs a, int kind, int h, i
 // One row a workgroup, one item a thread (rows of 128 to 1024 items). Position and slot are asked for before the tensors:
 // memory returns in order, so the angles are computed while the tensors fly. They go through the vector path, for
 // which a zero that the compiler cannot see through stands in: as the scalar loads it makes of a workgroup's one slot
-// and position, 14449 rows take 46.5 us instead of 45.8. (Two rows a workgroup: 45.7 us, and 9.2 instead of 8.6 for 2161 rows into an
-// E4M3 pool; three rows are slower throughout.)
+// and position, 14449 rows take 46.5 us instead of 45.8. (Two rows a workgroup: 45.7 us, and 9.2 instead of 8.6 for 2161
+// rows into an E4M3 pool; three rows are slower throughout.)
 template <int kHd, int kFmt, bool kStream>
 __global__ __launch_bounds__(kAppendThreads) void append_row(AppendArgs a, FreqTable freqs) {
     constexpr int kItems = kHd / 16, kHalf = kHd / 2;
