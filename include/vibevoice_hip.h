@@ -674,6 +674,8 @@ vv_status_t vv_kv_page_map_dev(int* page_table, int first, int n, const int* pag
  *   counts[3]              the balance of pages: *n_free less all that were asked for up to the last sequence served
  *                          (equal to *n_free_out unless a sequence before that was refused for want of pages; below
  *                          zero by what was missing), rows in use (row_starts[n_seqs]), sequences refused
+ * n_seqs <= 0 is no work: VV_OK and nothing is written, so positions and slots are still an earlier step's and must not be
+ * appended by (give n_seqs = 1 with a negative length, or skip the step).
  * free_pages is not written: a finished sequence's pages return by being written from free_pages[*n_free] on.
  * lens_out may be cache_lens and n_free_out may be n_free (a captured step that advances itself); one workgroup then
  * fills all rows (193 sequences with 2048 rows 13 us instead of 6, 32068 rows 104 instead of 5). Other overlaps are the caller's mistake; lens_out == new_lens and counts == n_free or n_free_out are

@@ -3,7 +3,10 @@ page, a tail or a single position, and a slot of a fixed pool that stands by kee
 import numpy as np
 import pytest
 
-from batch_util import (PAGE, attend, attend_bound_lifted, census, census_bound, pages_of, plan, slots_of)
+from __graft_entry__ import load_device
+from batch_util import PAGE, attend, attend_bound_lifted, census, census_bound, pages_of, plan, slots_of
+
+dev = load_device()
 
 
 def test_a_slot_that_stands_by_keeps_its_row():
@@ -15,6 +18,16 @@ def test_a_slot_that_stands_by_keeps_its_row():
     assert got["lens"].tolist() == [11, -1, -21, 64] and got["counts"].tolist() == [2, 4, 2]
     assert got["slots"].tolist() == [4 * PAGE + 10, -1, -1, 6 * PAGE + 63]
     assert np.array_equal(got["tables"], tables) and got["n_free"] == 2
+
+
+def test_no_sequences_are_no_work():
+    """VV_OK, and nothing is written: positions, slots and the rest keep what they held (host memory here: no launch)."""
+    held = [np.full(8, -77, np.int64) for _ in range(6)]
+    lens, starts, positions, slots, left, counts = (x.ctypes.data for x in held)
+    for n in (0, -1):
+        assert dev.vv_kv_page_plan_dev(lens, lens, n, lens, 4, lens, left, lens, starts, positions, slots, 8, left, counts,
+                                       None) == dev.VV_OK
+    assert all((x == -77).all() for x in held)
 
 
 def draw(n, nq, nkv, hd, rng, sharp=2.0):
