@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from batch_util import PAGE, attend, attend_bound_lifted, census, census_bound, pages_of, slots_of
-from gpu_util import dev, ok
+from gpu_util import dev, ok, stream
 from test_gpu_batch_serving import E4M3, E5M2, FP16, TORCH_FP8, Pool, ints, raw
 from test_gpu_batch_serving import test_append_against_the_separate_calls as append_against_the_separate_calls
 
@@ -148,3 +148,21 @@ def test_two_captured_steps_share_a_scratch():
             assert np.array_equal(raw(x.call()), w)
     for _, _, _, graph, _ in held:
         dev.vv_dev_graph_destroy(graph)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,fmt", [(28, 4, 128, FP16), (14, 2, 64, FP16), (28, 4, 128, E4M3), (6, 3, 96, FP16)])
+def test_attend_into_an_output_off_any_alignment(nq, nkv, hd, fmt):
+    """Only q, the stores and the scratch have an alignment to keep: out at two bytes, lengths and tables at four."""
+    p = Pool([3000, 0, 65, 700, 1], nq, nkv, hd, fmt=fmt, seed=44)
+    want, n = raw(p.call()), len(p.lens)
+    lens, tables = (torch.cat([ints([-5]), ints(x).flatten()]) for x in (p.lens, p.tables))
+    out = torch.full((n * nq * hd + 2,), float("nan"), dtype=torch.float16, device="cuda")
+    size = dev.vv_attn_decode_batch_scratch_bytes(n, nq, nkv, hd)
+    scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
+    view = dev.KvView(k=p.store[0].data_ptr(), v=p.store[1].data_ptr(), k_meta=None, v_meta=None,
+                      page_table=tables.data_ptr() + 4, format=fmt, n_kv_heads=nkv, head_dim=hd)
+    torch.cuda.synchronize()
+    ok(dev.vv_attn_decode_batch(2, p.q.data_ptr(), C.addressof(view), out.data_ptr() + 2, nq, n, lens.data_ptr() + 4,
+                                p.max_pages, p.n_pages, scratch.data_ptr(), size, stream()))
+    assert np.array_equal(raw(out[1:-1]).reshape(want.shape), want)
+    assert torch.isnan(out[0]) and torch.isnan(out[-1])
