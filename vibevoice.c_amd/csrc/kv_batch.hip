@@ -172,8 +172,9 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan(PlanArgs a) {
 // what of them is still cached is worth more than the hint (4096 rows: 12.5 us, 14.9 with it; 14449 rows 45.8 and 45.1).
 // The kernel of short and of very long rows stores ordinarily at every size: at 14 + 2 heads of 64 with the hint, 1000 to
 // 4096 rows are the same, 14449 rows 14.4 us instead of 13.6, and launches past 250 MB gain (60000 rows 55.9 instead of
-// 60.4; 4000 rows of 100 + 16 heads of 128 50.0 instead of 54.7). Measured at 28 + 4 heads of 128 with biases: 16 rows 3.0 us, 2161 rows into an E4M3 pool 8.6, 4096 rows 12.5 (6.0 TB/s), 14449 rows
-// 46 us (5.8 TB/s), into an E4M3 pool 45.6.
+// 60.4; 4000 rows of 100 + 16 heads of 128 50.0 instead of 54.7). Measured at 28 + 4 heads of 128 with
+// biases: 16 rows 3.0 us, 2161 rows into an E4M3 pool 8.6, 4096 rows 12.5 (6.0 TB/s), 14449 rows 46 us (5.8 TB/s), into
+// an E4M3 pool 45.6.
 struct AppendArgs {
     const h16* q;
     const h16* k;
